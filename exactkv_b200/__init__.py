@@ -4,16 +4,20 @@ and the page encoder that writes it — behind the reference's Python API.
 
 Same public names as the reference package (exactkv/__init__.py:3-12).
 """
-from .cache import CompressedKV, BF16KV, check_overflow
+from .cache import CompressedKV, BF16KV, PagedCompressedKV, check_overflow
 from .attention import decode_attention
 from .codec import encode_reference, decode_reference, bits_per_value
 from .kernels import attention_compressed, attention_reference, decode_to_bf16, encode_pages
+from .kernels import attention_prefill, attention_prefill_paged, attention_prefill_reference_paged
+from .kernels import rope_append_paged, rope_append_reference_paged, rope_table
 from . import kernels
 
 __version__ = "0.1.0"
-__all__ = ["CompressedKV", "BF16KV", "check_overflow", "decode_attention", "Engine",
+__all__ = ["CompressedKV", "BF16KV", "PagedCompressedKV", "check_overflow", "decode_attention", "Engine",
            "encode_reference", "decode_reference", "bits_per_value",
-           "attention_compressed", "attention_reference", "decode_to_bf16", "encode_pages", "kernels"]
+           "attention_compressed", "attention_reference", "decode_to_bf16", "encode_pages",
+           "attention_prefill", "attention_prefill_paged", "attention_prefill_reference_paged", "rope_append_paged",
+           "rope_append_reference_paged", "rope_table", "kernels"]
 
 
 def __getattr__(name):

@@ -16,8 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libexactkv_b200.so")
-SOURCES = ["exk_host.cu", "exk_attention.cu", "exk_codec.cu", "exk_noalloc.cu"]
-HEADERS = ["exk_device.cuh", "exk_host.h", os.path.join("..", "..", "include", "exactkv_b200.h")]
+SOURCES = ["exk_host.cu", "exk_attention.cu", "exk_codec.cu", "exk_noalloc.cu", "exk_paged.cu", "exk_prefill.cu"]
+HEADERS = ["exk_device.cuh", "exk_encode.cuh", "exk_host.h", os.path.join("..", "..", "include", "exactkv_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -236,6 +236,70 @@ class CompressedKV:
         return torch.tensor(self.lens, dtype=torch.int32, device=self.dev)
 
 
+class PagedCompressedKV:
+    """A pool of `pages` 16-token pages of one layer's keys (or values) in the
+    compressed format, H KV heads, head dim 128, for up to `max_seqs` sequences
+    that are being written: each has a tail slot, where its open page is kept
+    raw. Written by kernels.rope_append_paged, read by kernels.attention_paged
+    and kernels.attention_prefill_paged, all through int32 block tables that the
+    caller keeps. `reserve`: initial raw-pool slots as a fraction of all rows."""
+
+    def __init__(self, pages, H, D, max_seqs, device="cuda", reserve=0.01):
+        if pages <= 0 or max_seqs <= 0 or H <= 0 or D != 128:
+            raise ValueError("pages, H and max_seqs must be positive and D = 128 (Qwen2/2.5/3, Llama-3 family)")
+        self.B, self.TS, self.H, self.D = 1, pages * P, H, D       # the pages as one long sequence of rows
+        self.dev = torch.device(device)
+        u8 = dict(dtype=torch.uint8, device=self.dev)
+        i32 = dict(dtype=torch.int32, device=self.dev)
+        self.sm = torch.zeros(1, pages * P, H, D, **u8)
+        self.code = torch.zeros(1, pages * P, H, D // 2, **u8)
+        self.base = torch.zeros(1, pages, H, D, **u8)
+        self.rowmask = torch.zeros(1, pages, H, **i32)
+        self.rowoff = torch.zeros(1, pages, H, **i32)
+        self.cnt = torch.zeros(1, **i32)
+        self.pool = RawPool(max_seqs, H, D, max(64, int(pages * P * H * reserve)), self.dev)
+        self._bind()
+
+    @property
+    def raw(self):
+        return self.pool.rows
+
+    @property
+    def cap(self):
+        return self.pool.cap
+
+    def _bind(self):
+        self._view = CView(self.sm.data_ptr(), self.code.data_ptr(), self.base.data_ptr(), self.rowmask.data_ptr(),
+                           self.rowoff.data_ptr(), self.pool.rows.data_ptr(), self.pool.rows.shape[0])
+
+    def kernel_view(self):
+        return self._view
+
+    def buffers(self):
+        return dict(shape=(1, self.TS, self.H, self.D), sm=self.sm, code=self.code, base=self.base,
+                    rowmask=self.rowmask, rowoff=self.rowoff, raw=self.pool.rows, cnt=self.cnt, cap=self.pool.cap)
+
+    def nbytes(self):
+        return sum(t.numel() * t.element_size()
+                   for t in (self.sm, self.code, self.base, self.rowmask, self.rowoff, self.pool.rows))
+
+    def ensure_headroom(self, tokens):
+        """Before `tokens` more tokens are appended: one sync to read the slot counter,
+        then grow so that even `tokens` tokens of nothing but raw rows fit (they and
+        the rows already in open pages: 16 for each sequence). Returns True when the
+        pool moved (a captured graph must be captured again)."""
+        used = int(self.cnt.item())
+        need = used + (tokens + P * self.pool.nseq) * self.H
+        old = self.pool.cap
+        if need <= old:
+            return False
+        self.pool.enlarge(used, need)
+        self._bind()
+        # entries at or past the old capacity are open pages': they move with the tail slots
+        self.rowoff += (self.rowoff >= old).int() * (self.pool.cap - old)
+        return True
+
+
 class BF16KV:
     """Uncompressed bf16 cache [B, TS, H, D] with the same interface."""
 

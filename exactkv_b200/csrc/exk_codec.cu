@@ -16,22 +16,13 @@
 #include <algorithm>
 
 #include "exk_device.cuh"
+#include "exk_encode.cuh"
 #include "exk_host.h"
 
 namespace exk {
 
 constexpr int kEncWarps = 8;
 constexpr int kScanThreads = 1024;
-
-// The kernels after the first of a call are programmatic dependents of the
-// kernel before them on the stream (launch_after): they may become resident
-// while it runs its last wave, which hides their launch latency, and wait in
-// after_prior() until it has completed and its writes are visible (a no-op
-// after an ordinary launch). allow_dependents() lets them be scheduled.
-__device__ __forceinline__ void after_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void allow_dependents() {
-  if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
 
 struct EncArgs {
   const uint16_t* src;
@@ -90,45 +81,6 @@ __device__ __forceinline__ int64_t page_index(const EncArgs& a, int pg0, int ph,
   pg = (ph / a.H) % a.npg;
   bi = ph / (a.H * a.npg);
   return (static_cast<int64_t>(a.b0 + bi) * a.NP + pg0 + pg) * a.H + hk;
-}
-
-// Constants the compiler cannot see (2^25, 2^24, 1, 2), so that shifts and
-// lane-wise adds of the encoder become multiplies on the FMA pipe: the encoder
-// keeps the ALU pipe busy. A lane-wise add is a plain 32-bit add when neither
-// 16-bit lane can carry into the next: the lanes then hold 0x8000 + e - b.
-static __constant__ uint32_t c_fma[5] = {1u << 25, 1u << 24, 1u, 2u, 16u};
-
-__device__ __forceinline__ uint32_t mulhi(uint32_t x, uint32_t k) {
-  uint32_t d;
-  asm("mul.hi.u32 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(k));
-  return d;
-}
-__device__ __forceinline__ uint32_t mad_lo(uint32_t x, uint32_t k, uint32_t y) {
-  uint32_t d;
-  asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(k), "r"(y));
-  return d;
-}
-
-// Two 16-bit lanes per word (PTX integer SIMD; add wraps within each lane).
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t x, uint32_t y) {
-  uint32_t d;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
-  return d;
-}
-__device__ __forceinline__ uint32_t min_u16x2(uint32_t x, uint32_t y) {
-  uint32_t d;
-  asm("min.u16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
-  return d;
-}
-__device__ __forceinline__ uint32_t max_s16x2(uint32_t x, uint32_t y) {
-  uint32_t d;
-  asm("max.s16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
-  return d;
-}
-__device__ __forceinline__ uint32_t add_u16x2(uint32_t x, uint32_t y) {
-  uint32_t d;
-  asm("add.u16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
-  return d;
 }
 
 template <bool VEC>

@@ -18,6 +18,23 @@ int make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* ptr, u
 // keeps its own notion of the current device) and returns its SM count.
 int use_device(int device, int* num_sms);
 
+// The caller's current device, put back when the entry point returns.
+struct DeviceScope {
+  int device = -1;
+  DeviceScope() {
+    if (cudaGetDevice(&device) != cudaSuccess) {
+      (void)cudaGetLastError();
+      device = -1;
+    }
+  }
+  ~DeviceScope() {
+    int now = -1;
+    if (device >= 0 && cudaGetDevice(&now) == cudaSuccess && now != device) cudaSetDevice(device);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // 0 if kernels may store through p: device or managed memory, or pinned host

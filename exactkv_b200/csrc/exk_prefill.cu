@@ -1,0 +1,789 @@
+// Causal attention of many query tokens per sequence (sm_100a): packed prompts
+// over their own keys, or a prompt's chunk over the pages of a paged cache.
+//
+// Query i of a sequence of n queries and L keys sees keys j <= i + L - n:
+//   o_i = sum_j softmax_j(q_i k_j / sqrt(128)) v_j ,  0 where it sees none.
+//
+// One CTA takes 256 rows of one KV head's group: a row is a (token, query head
+// of the group) pair, so the G = Hq / Hkv heads that share keys share the
+// CTA's key tiles, and 256 / G consecutive tokens keep the diagonal narrow. It
+// streams tiles of 128 keys from the diagonal down: S = Q K^T (tcgen05, K-major
+// operands in shared memory, S in TMEM), one thread per row for the running
+// maximum, P = 2^(s - m) in bf16 back into TMEM over S, O += P V (P from TMEM, V
+// MN-major as the TMA left it). Two 128-row tiles alternate, so the tensor
+// core works on one while the other's softmax runs.
+#include <algorithm>
+
+#include "exk_device.cuh"
+#include "exk_encode.cuh"
+#include "exk_host.h"
+
+namespace exk {
+
+namespace {
+
+constexpr int kTile = 128;                 // rows of a query tile, keys of a key tile
+constexpr int kHalf = kTile * 128;         // bytes of one operand half: 128 rows x 64 channels bf16
+constexpr int kOperand = 2 * kHalf;        // one operand tile
+constexpr int kSlots = 4;                  // key/value ring: K, V, K, V, ...
+constexpr int kPrefillThreads = 384;       // warps 0-3, 4-7: softmax; 8: MMA; 9: TMA; 10, 11: values of masked tiles
+constexpr int kRegsSoftmax = 208, kRegsOther = 80;
+constexpr float kRescale = 8.f;            // a row's maximum may grow by 2^8 before O is rescaled
+
+struct PrefillArgs {
+  const int32_t* cu_q;
+  const int32_t* cu_k;         // packed keys, or null
+  const int32_t* lens;         // keys of each sequence where cu_k is null
+  const int32_t* block_table;  // pages of the keys, or null: sequence b's rows start at b * k_stride
+  int64_t k_stride;
+  const uint16_t* v;           // the values again, for non-finite ones under a mask
+  int64_t v_st, v_sh;
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  float* po;                   // partials [N * Hq, ns, 128], [N * Hq, ns] (ns > 1)
+  float* pm;
+  float* pl;
+  int32_t* status;
+  int N, Nk, B, Hq, Hkv, G, tpt;  // tpt: tokens of a query tile
+  int max_pages, pool_pages, ns, slots;
+  float scale;                 // log2(e) / sqrt(128)
+};
+
+struct PrefillMaps {
+  CUtensorMap q, k, v;
+};
+
+// ---------------------------------------------------------------- tcgen05
+
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Arrives on `bar` when every tcgen05 operation this thread issued before has completed.
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
+}
+
+// D[tmem] (+)= A[smem] B[smem]; both bf16, fp32 accumulation.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem].
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// 32 columns of the calling warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(v[0]),
+      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+      "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(addr)
+      : "memory");
+}
+
+// Shared-memory operand descriptors, 128-byte swizzle, tiles as TMA leaves
+// them: 128-byte rows (64 channels), eight rows to a 1024-byte swizzle block.
+// K-major (Q, K: the contraction runs along the row): groups of eight rows
+// 1024 bytes apart; 16 channels are 32 bytes further. MN-major (V: the
+// contraction runs down the rows): the second half of the channels kHalf
+// bytes on, the next eight keys 1024; 16 keys are 2048 bytes further.
+constexpr uint64_t kDescBase = (uint64_t{1} << 46) | (uint64_t{2} << 61);
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
+  return kDescBase | (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 16) | ((addr & 0x3FFFF) >> 4);
+}
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
+  return kDescBase | (uint64_t{1024 >> 4} << 32) | (uint64_t{kHalf >> 4} << 16) | ((addr & 0x3FFFF) >> 4);
+}
+// fp32 D, bf16 A and B, M = N = 128; bit 16: B is MN-major.
+constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kTile / 8) << 17) | ((kTile / 16) << 24);
+constexpr uint32_t kIdescMN = kIdesc | (1u << 16);
+
+// ---------------------------------------------------------------- one CTA's work
+
+struct Work {
+  int first, n;     // the sequence's first packed query, its queries
+  int L;            // its keys
+  int64_t krow;     // its first key row (not paged)
+  int b, hk;
+  int tok0;         // first token of the CTA's rows
+  int tiles;        // query tiles in use: 1 or 2
+  int keys;         // keys that the last row sees
+  int t0, t1;       // key tiles [t0, t1) of this split
+  int low;          // keys that the first row sees (may be negative): tiles past it are masked
+};
+
+// Slot s of the call -> sequence and 256-row block. Sequence b's blocks take
+// slots cu[b] / T + b, + 1, ... with T = 2 tpt tokens a block: n tokens need
+// at most (n + T - 1) / T, which never reaches sequence b + 1's first slot.
+__device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int lane, Work& w) {
+  const int T = 2 * a.tpt;
+  const int split = item % a.ns;
+  w.hk = (item / a.ns) % a.Hkv;
+  const int slot = a.slots - 1 - item / (a.ns * a.Hkv);  // long rows of keys first
+  int b = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const bool before = b0 + lane < a.B && __ldg(a.cu_q + b0 + lane + 1) / T + b0 + lane + 1 <= slot;
+    b += __popc(__ballot_sync(0xFFFFFFFFu, before));
+  }
+  if (b >= a.B) return false;
+  w.b = b;
+  w.first = __ldg(a.cu_q + b);
+  w.n = __ldg(a.cu_q + b + 1) - w.first;
+  if (w.first < 0 || w.n <= 0 || w.first > a.N - w.n) return false;
+  w.tok0 = (slot - (w.first / T + b)) * T;
+  if (w.tok0 < 0 || w.tok0 >= w.n) return false;
+  if (a.cu_k != nullptr) {
+    w.krow = __ldg(a.cu_k + b);
+    w.L = __ldg(a.cu_k + b + 1) - static_cast<int>(w.krow);
+    if (w.krow < 0 || w.L < 0 || w.krow > a.Nk - w.L) w.L = 0;
+  } else {
+    w.krow = b * a.k_stride;
+    w.L = __ldg(a.lens + b);
+    const int most = a.block_table != nullptr ? a.max_pages * kP : static_cast<int>(a.k_stride);
+    w.L = max(0, min(w.L, most));
+  }
+  w.tiles = w.n - w.tok0 > a.tpt ? 2 : 1;
+  w.low = w.L - w.n + w.tok0 + 1;
+  w.keys = max(0, w.L - w.n + min(w.tok0 + T, w.n));
+  const int nt = (w.keys + kTile - 1) / kTile;
+  const int per = (nt + a.ns - 1) / a.ns;
+  w.t0 = min(nt, split * per);
+  w.t1 = min(nt, w.t0 + per);
+  return true;
+}
+
+__device__ __forceinline__ bool tile_masked(const Work& w, int j) { return (j + 1) * kTile > w.low; }
+
+// Waits that end: after kWaitLimitNs, or at once when another role gave up.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*stop != 0) return false;
+    if (globaltimer() - t0 > kWaitLimitNs) {
+      *stop = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// bar_wait by a whole warp, with one answer for all lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, stop));
+}
+
+struct __align__(8) Bars {
+  uint64_t q_full[2], kv_full[kSlots], kv_empty[kSlots], v_ok[kSlots], s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int stop, bad;
+};
+
+constexpr int kPrefillSmem = 2 * kOperand + kSlots * kOperand + static_cast<int>(sizeof(Bars)) + 1024;
+
+__global__ void __launch_bounds__(kPrefillThreads, 1)
+    prefill_kernel(const __grid_constant__ PrefillArgs a, const __grid_constant__ PrefillMaps maps) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sq = smem;
+  uint8_t* ring = smem + 2 * kOperand;
+  Bars* bars = reinterpret_cast<Bars*>(ring + kSlots * kOperand);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* stop = &bars->stop;
+
+  Work w;
+  if (!load_work(a, blockIdx.x, lane, w)) return;  // the whole CTA
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], kTile);
+      mbar_init(&bars->o_full[i], 1);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&bars->kv_full[i], 1);
+      mbar_init(&bars->kv_empty[i], 1);
+      mbar_init(&bars->v_ok[i], 64);
+    }
+    bars->stop = bars->bad = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) tmem_alloc(&bars->tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+  const int nt = w.t1 - w.t0;  // key tiles, from w.t1 - 1 down
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int x = warp >> 2;                 // query tile
+    const int r = threadIdx.x & 127;         // row
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    const uint32_t ts = tmem + lanes + x * kTile, to = tmem + lanes + 2 * kTile + x * kTile;
+    const int tok = w.tok0 + x * a.tpt + r / a.G;
+    const bool valid = r < a.G * a.tpt && tok < w.n;
+    const int lim = w.L - w.n + tok;         // last key the row sees
+    float m = -INFINITY, l = 0.f;
+    if (x < w.tiles) {
+      for (int it = 0; it < nt; ++it) {
+        const int j = w.t1 - 1 - it;
+        if (!warp_wait(&bars->s_full[x], it & 1, stop)) break;
+        tc_fence_after();
+        uint32_t s[kTile];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
+        tc_wait_ld();
+        if (tile_masked(w, j)) {
+          const int seen = lim - j * kTile;
+#pragma unroll
+          for (int i = 0; i < kTile; ++i)
+            if (i > seen) s[i] = 0xFF800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+        if (it == 0) {
+          m = top;
+        } else if (__any_sync(0xFFFFFFFFu, top > m + kRescale)) {
+          // S is complete, so the tensor core has finished O += P V of the tile before
+          const float mn = fmaxf(m, top);
+          const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
+          l *= f;
+          m = mn;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(to + 32 * c, o);
+          }
+        }
+        const float off = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t p[kTile / 2];
+#pragma unroll
+        for (int i = 0; i < kTile; i += 2) {
+          const float p0 = ex2(fmaf(__uint_as_float(s[i]), a.scale, off));
+          const float p1 = ex2(fmaf(__uint_as_float(s[i + 1]), a.scale, off));
+          sum[(i >> 1) & 3] += p0 + p1;
+          p[i >> 1] = pack_bf16x2(p0, p1);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st32(ts, p);
+        tmem_st32(ts + 32, p + 32);
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full[x]);
+      }
+      const bool have = nt > 0 && warp_wait(&bars->o_full[x], 0, stop);
+      tc_fence_after();
+      const int h = w.hk * a.G + r % a.G;
+      const int64_t row = static_cast<int64_t>(w.first + tok) * a.Hq + h;
+      if (a.ns > 1 && valid) {
+        const int split = blockIdx.x % a.ns;
+        a.pm[row * a.ns + split] = have ? m : -INFINITY;
+        a.pl[row * a.ns + split] = have ? l : 0.f;
+      }
+      const float inv = a.ns > 1 ? 1.f : (have && l > 0.f ? 1.f / l : (l != l ? l : 0.f));
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        if (have) {
+          tmem_ld32(to + 32 * c, o);
+          tc_wait_ld();
+        }
+        if (!valid) continue;
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = have && !(l == 0.f) ? __uint_as_float(o[i]) * inv : 0.f;
+        if (bars->bad != 0) {
+          // a masked tile held values that are not finite: they were left out of
+          // the product and reach the rows that see them here
+          for (int j = w.t0; j < w.t1; ++j) {
+            if (!tile_masked(w, j)) continue;
+            for (int t = j * kTile; t < min((j + 1) * kTile, lim + 1); ++t) {
+              int64_t vrow = w.krow + t;
+              if (a.block_table != nullptr) {
+                const int pg = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + t / kP);
+                if (pg < 0 || pg >= a.pool_pages) continue;
+                vrow = static_cast<int64_t>(pg) * kP + t % kP;
+              }
+              const uint16_t* vp = a.v + vrow * a.v_st + w.hk * a.v_sh + 32 * c;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if ((vp[i] & 0x7F80) == 0x7F80) f[i] += __uint_as_float(static_cast<uint32_t>(vp[i]) << 16);
+            }
+          }
+        }
+        if (a.ns > 1) {
+          float4* d = reinterpret_cast<float4*>(a.po + (row * a.ns + blockIdx.x % a.ns) * kD + 32 * c);
+          if (have) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+          }
+        } else {
+          uint4* d = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(w.first + tok) * a.o_st + h * a.o_sh + 32 * c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            d[i] = make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
+                              pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+        }
+      }
+    }
+    tc_fence_before();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == 8 && nt > 0) {
+      // ---- MMA: K of tile `it` is ring entry 2 it, V is 2 it + 1
+      auto qk = [&](int x, int slot) {
+        if (lane == 0) {
+          const uint32_t qa = smem_addr(sq) + x * kOperand, ka = smem_addr(ring) + slot * kOperand;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
+            mma_ss(tmem + x * kTile, desc_kmajor(qa + off), desc_kmajor(ka + off), kIdesc, k > 0);
+          }
+          tc_commit(&bars->s_full[x]);
+        }
+        __syncwarp();
+      };
+      bool ok = true;
+      for (int x = 0; x < w.tiles && ok; ++x) {
+        ok = warp_wait(&bars->q_full[x], 0, stop) && (x > 0 || warp_wait(&bars->kv_full[0], 0, stop));
+        tc_fence_after();
+        if (ok) qk(x, 0);
+      }
+      if (ok && lane == 0) tc_commit(&bars->kv_empty[0]);
+      for (int it = 0; it < nt && ok; ++it) {
+        const int ve = 2 * it + 1, ke = 2 * it + 2;
+        const int vs = ve % kSlots, ks = ke % kSlots;
+        const uint32_t vph = (ve / kSlots) & 1, kph = (ke / kSlots) & 1;
+        for (int x = 0; x < w.tiles && ok; ++x) {
+          if (x == 0) {
+            // the masked tiles come first, so the k-th use of v_ok[vs] is the k-th use of the slot
+            ok = warp_wait(tile_masked(w, w.t1 - 1 - it) ? &bars->v_ok[vs] : &bars->kv_full[vs], vph, stop);
+          }
+          ok = ok && warp_wait(&bars->p_full[x], it & 1, stop);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t va = smem_addr(ring) + vs * kOperand;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              mma_ts(tmem + 2 * kTile + x * kTile, tmem + x * kTile + 8 * k, desc_mnmajor(va + 2048 * k), kIdescMN,
+                     it > 0 || k > 0);
+            if (x == w.tiles - 1) tc_commit(&bars->kv_empty[vs]);
+            if (it == nt - 1) tc_commit(&bars->o_full[x]);
+          }
+          __syncwarp();
+          if (it < nt - 1) {
+            if (x == 0) ok = warp_wait(&bars->kv_full[ks], kph, stop);
+            if (ok) qk(x, ks);
+          }
+        }
+        if (ok && it < nt - 1 && lane == 0) tc_commit(&bars->kv_empty[ks]);
+      }
+    } else if (warp == 9 && nt > 0) {
+      // ---- TMA
+      const int tile_bytes = 64 * 2 * a.G * a.tpt;
+      if (lane == 0) {
+        prefetch_tmap(&maps.q);
+        prefetch_tmap(&maps.k);
+        prefetch_tmap(&maps.v);
+        for (int x = 0; x < w.tiles; ++x) {
+          mbar_arrive_expect_tx(&bars->q_full[x], 2 * tile_bytes);
+          for (int c = 0; c < 2; ++c)
+            tma_load_3d(sq + x * kOperand + c * kHalf, &maps.q, 64 * c, w.hk * a.G, w.first + w.tok0 + x * a.tpt,
+                        &bars->q_full[x]);
+        }
+      }
+      for (int e = 0; e < 2 * nt; ++e) {
+        const int slot = e % kSlots, j = w.t1 - 1 - e / 2;
+        if (e >= kSlots && !warp_wait(&bars->kv_empty[slot], ((e / kSlots) & 1) ^ 1, stop)) break;
+        const CUtensorMap* map = (e & 1) == 0 ? &maps.k : &maps.v;
+        uint8_t* dst = ring + slot * kOperand;
+        if (a.block_table == nullptr) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars->kv_full[slot], kOperand);
+            for (int c = 0; c < 2; ++c)
+              tma_load_3d(dst + c * kHalf, map, 64 * c, w.hk, static_cast<int>(w.krow) + j * kTile, &bars->kv_full[slot]);
+          }
+        } else {
+          // one lane per page; pages past the keys are not loaded (their columns are masked)
+          const int pages = min(kTile / kP, (w.keys - j * kTile + kP - 1) / kP);
+          int row = 0;
+          if (lane < pages) {
+            const int pg = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + j * (kTile / kP) + lane);
+            if (pg >= 0 && pg < a.pool_pages) {
+              row = pg * kP;
+            } else {
+              set_status(a.status, EXK_S_PAGE_INDEX);
+              row = a.pool_pages * kP;  // outside the map: zeros
+            }
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[slot], pages * (2 * 64 * 2 * kP));
+          __syncwarp();
+          if (lane < pages) {
+            for (int c = 0; c < 2; ++c)
+              tma_load_3d(dst + c * kHalf + lane * (kP * 128), map, 64 * c, w.hk, row, &bars->kv_full[slot]);
+          }
+        }
+        __syncwarp();
+      }
+    } else if (warp >= 10 && nt > 0) {
+      // ---- values of masked tiles: rows past the last key become zeros, and so do
+      // values that are not finite (0 x inf would reach rows that do not see them)
+      for (int it = 0; it < nt && tile_masked(w, w.t1 - 1 - it); ++it) {
+        const int j = w.t1 - 1 - it, ve = 2 * it + 1, vs = ve % kSlots;
+        if (!bar_wait(&bars->kv_full[vs], (ve / kSlots) & 1, stop)) break;
+        const int t = threadIdx.x - 320;
+        uint4* v = reinterpret_cast<uint4*>(ring + vs * kOperand);
+        bool bad = false;
+        const int rows = w.keys - j * kTile;  // keys of the tile that some row sees
+        for (int i = t; i < kOperand / 16; i += 64) {
+          const int row = (i >> 3) & (kTile - 1);
+          if (row >= rows) {
+            v[i] = make_uint4(0, 0, 0, 0);
+          } else {
+            uint4 u = v[i];
+            uint32_t e[4] = {u.x, u.y, u.z, u.w};
+            bool hit = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if ((e[k] & 0x7F80u) == 0x7F80u) {
+                e[k] &= 0xFFFF0000u;
+                hit = true;
+              }
+              if ((e[k] & 0x7F800000u) == 0x7F800000u) {
+                e[k] &= 0xFFFFu;
+                hit = true;
+              }
+            }
+            if (hit) v[i] = make_uint4(e[0], e[1], e[2], e[3]);
+            bad |= hit;
+          }
+        }
+        if (bad) *const_cast<volatile int*>(&bars->bad) = 1;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&bars->v_ok[vs]);
+      }
+    }
+  }
+  __syncthreads();
+  if (*stop != 0) {
+    // a wait ran out: what is in flight (copies of at most 192 KB, products of a
+    // tile) ends long before this pause does, and nothing more is issued
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 2000000) {
+    }
+    if (threadIdx.x == 0) set_status(a.status, EXK_S_FULL_TIMEOUT);
+    __syncthreads();
+  }
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+// Partials of ns splits of each row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M),
+// 0 for a row without keys; rows of no sequence are left alone. One warp per row.
+__global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constant__ PrefillArgs a) {
+  after_prior();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= static_cast<int64_t>(a.N) * a.Hq) return;
+  const int tok = static_cast<int>(row / a.Hq);
+  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.B)) return;
+  const float* pm = a.pm + row * a.ns;
+  const float* pl = a.pl + row * a.ns;
+  float M = -INFINITY;
+  for (int s = lane; s < a.ns; s += 32) M = fmaxf(M, pm[s]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
+  float den = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < a.ns; ++s) {
+    const float ms = pm[s], ls = pl[s];
+    if (ms == -INFINITY && ls == 0.f) continue;  // the split holds no key of this row
+    const float f = M == -INFINITY ? 1.f : ex2(ms - M);
+    const float4 o = reinterpret_cast<const float4*>(a.po + (row * a.ns + s) * kD)[lane];
+    den += f * ls;
+    acc.x += f * o.x;
+    acc.y += f * o.y;
+    acc.z += f * o.z;
+    acc.w += f * o.w;
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  uint16_t* d = a.out + tok * a.o_st + (row % a.Hq) * a.o_sh;
+  reinterpret_cast<uint2*>(d)[lane] =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+}
+
+// Coded pages of the sequences into bf16 rows b * k_stride + position: the
+// pages' keys (blockIdx.y 0) and values (1), a warp per (page, KV head).
+struct Unpack {
+  exk_cview c[2];
+  uint16_t* out[2];
+  const int32_t* block_table;
+  const int32_t* lens;
+  int32_t* status;
+  int64_t k_stride;
+  int B, Hkv, max_pages, pool_pages, pages;  // pages: k_stride / 16
+};
+
+__global__ void __launch_bounds__(256) unpack_kernel(const __grid_constant__ Unpack u) {
+  allow_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t ph = static_cast<int64_t>(blockIdx.x) * 8 + warp;
+  const int h = static_cast<int>(ph % u.Hkv);
+  const int pg = static_cast<int>((ph / u.Hkv) % u.pages);
+  const int64_t b = ph / (static_cast<int64_t>(u.Hkv) * u.pages);
+  if (b >= u.B) return;
+  const int L = min(__ldg(u.lens + b), static_cast<int>(u.k_stride));
+  if (pg * kP >= L) return;
+  const int pool = __ldg(u.block_table + b * u.max_pages + pg);
+  const exk_cview& c = u.c[blockIdx.y];
+  const int q = lane & 15, th = lane >> 4;
+  uint16_t* out = u.out[blockIdx.y] + ((b * u.k_stride + static_cast<int64_t>(pg) * kP + 8 * th) * u.Hkv + h) * kD;
+  const bool bad = pool < 0 || pool >= u.pool_pages;
+  if (bad) set_status(u.status, EXK_S_PAGE_INDEX);
+  const int64_t page = bad ? 0 : static_cast<int64_t>(pool) * u.Hkv + h;
+  const uint32_t rm = bad ? 0u : static_cast<uint32_t>(c.rowmask[page]) & 0xFFFFu;
+  const int32_t ro = bad ? 0 : c.rowoff[page];
+  const uint32_t bl = *reinterpret_cast<const uint32_t*>(c.base + page * kD + 4 * q);
+  const uint32_t bh = *reinterpret_cast<const uint32_t*>(c.base + page * kD + 64 + 4 * q);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int tok = th * 8 + i;
+    uint32_t w0 = 0u, w1 = 0u, w2 = 0u, w3 = 0u;
+    if (pg * kP + tok >= L) break;
+    if (bad) {
+    } else if ((rm >> tok) & 1u) {
+      const int64_t ridx = static_cast<int64_t>(ro) + __popc(rm & ((1u << tok) - 1u));
+      if (ridx < 0 || ridx >= c.raw_rows) {
+        set_status(u.status, EXK_S_RAW_INDEX);
+      } else {
+        const uint16_t* r = c.raw + ridx * kD;
+        const uint2 lo = *reinterpret_cast<const uint2*>(r + 4 * q), hi = *reinterpret_cast<const uint2*>(r + 64 + 4 * q);
+        w0 = lo.x; w1 = lo.y; w2 = hi.x; w3 = hi.y;
+      }
+    } else {
+      const int64_t row = (static_cast<int64_t>(pool) * kP + tok) * u.Hkv + h;
+      const uint32_t sl = *reinterpret_cast<const uint32_t*>(c.sm + row * kD + 4 * q);
+      const uint32_t sh = *reinterpret_cast<const uint32_t*>(c.sm + row * kD + 64 + 4 * q);
+      const uint32_t cw = *reinterpret_cast<const uint32_t*>(c.code + row * (kD / 2) + 4 * q);
+      dec4(sl, lo_nibbles(cw), bl & 0x7F7F7F7Fu, bl, w0, w1);
+      dec4(sh, hi_nibbles(cw), bh & 0x7F7F7F7Fu, bh, w2, w3);
+    }
+    uint16_t* o = out + static_cast<int64_t>(i) * u.Hkv * kD;
+    *reinterpret_cast<uint2*>(o + 4 * q) = make_uint2(w0, w1);
+    *reinterpret_cast<uint2*>(o + 64 + 4 * q) = make_uint2(w2, w3);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+int64_t prefill_slots(int N, int B, int G) { return N / (2 * (kTile / G)) + static_cast<int64_t>(B); }
+
+int check_prefill(const exk_prefill* p) {
+  if (p == nullptr || p->q == nullptr || p->out == nullptr || p->cu_q == nullptr) return EXK_EARG;
+  if (p->N < 0 || p->B <= 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv != 0 || p->ns < 1 || p->ns > 256 ||
+      p->N > (1 << 28) || p->B > (1 << 24) || p->Hq > 4096)
+    return EXK_EARG;
+  if (p->Hq / p->Hkv > 16) return EXK_EHEADS;
+  if (p->ns > 1 && (p->po == nullptr || p->pm == nullptr || p->pl == nullptr)) return EXK_EARG;
+  if (!aligned16(p->q) || !aligned16(p->out) || !aligned16(p->po)) return EXK_EALIGN;
+  for (int64_t s : {p->q_st, p->q_sh, p->o_st, p->o_sh})
+    if (s % 8 != 0) return EXK_EALIGN;
+  if (p->q_st <= 0 || p->q_sh <= 0) return EXK_EARG;
+  return 0;
+}
+
+// Rows [rows, heads, 128] with element strides; box of `tokens` rows of `heads_box` heads, 64 channels.
+int make_rows_map(CUtensorMap* map, const uint16_t* p, int64_t rows, int heads, int64_t st, int64_t sh, int heads_box,
+                  int tokens) {
+  return make_tmap_3d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, kD, heads, rows, sh * 2, st * 2, 64, heads_box, tokens,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int launch_prefill(const exk_prefill* p, PrefillArgs& a, const uint16_t* k, int64_t k_st, int64_t k_sh, const uint16_t* v,
+                   int64_t v_st, int64_t v_sh, int64_t key_rows, int key_box, int32_t* status, cudaStream_t st) {
+  if (!aligned16(k) || !aligned16(v)) return EXK_EALIGN;
+  for (int64_t s : {k_st, k_sh, v_st, v_sh}) {
+    if (s % 8 != 0) return EXK_EALIGN;
+    if (s <= 0) return EXK_EARG;
+  }
+  a.cu_q = p->cu_q;
+  a.v = v;
+  a.v_st = v_st;
+  a.v_sh = v_sh;
+  a.out = p->out;
+  a.o_st = p->o_st;
+  a.o_sh = p->o_sh;
+  a.po = p->po;
+  a.pm = p->pm;
+  a.pl = p->pl;
+  a.status = status;
+  a.N = p->N;
+  a.B = p->B;
+  a.Hq = p->Hq;
+  a.Hkv = p->Hkv;
+  a.G = p->Hq / p->Hkv;
+  a.tpt = kTile / a.G;
+  a.ns = p->ns;
+  a.scale = p->qk_scale;
+  const int64_t slots = prefill_slots(p->N, p->B, a.G);
+  const int64_t grid = slots * p->Hkv * p->ns;
+  if (grid >= (int64_t{1} << 31)) return EXK_EARG;
+  a.slots = static_cast<int>(slots);
+  PrefillMaps maps;
+  int r;
+  if ((r = make_rows_map(&maps.q, p->q, p->N, p->Hq, p->q_st, p->q_sh, a.G, a.tpt)) != 0) return r;
+  if ((r = make_rows_map(&maps.k, k, key_rows, p->Hkv, k_st, k_sh, 1, key_box)) != 0) return r;
+  if ((r = make_rows_map(&maps.v, v, key_rows, p->Hkv, v_st, v_sh, 1, key_box)) != 0) return r;
+  const cudaError_t e = cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrefillSmem);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  prefill_kernel<<<static_cast<unsigned>(grid), kPrefillThreads, kPrefillSmem, st>>>(a, maps);
+  if ((r = launch_status()) != 0 || p->ns == 1) return r;
+  const int64_t rows = static_cast<int64_t>(p->N) * p->Hq;
+  prefill_merge_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(a);
+  return launch_status();
+}
+
+}  // namespace
+
+}  // namespace exk
+
+using namespace exk;
+
+extern "C" int exk_prefill_splits(int N, int B, int Hq, int Hkv, int64_t max_keys, int num_sms) {
+  if (N < 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_keys < 0 || num_sms <= 0) return EXK_EARG;
+  if (Hq / Hkv > 16) return EXK_EHEADS;
+  const int64_t items = prefill_slots(N, B, Hq / Hkv) * Hkv;
+  const int64_t tiles = (max_keys + kTile - 1) / kTile;
+  // whole waves of CTAs need no splits; else as many as fill the SMs once, of four key tiles at least
+  const int64_t fit = items > 0 ? num_sms / items : 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({fit, tiles / 4, 64})));
+}
+
+extern "C" int exk_attention_prefill(const exk_prefill* p, const uint16_t* k, int64_t k_st, int64_t k_sh,
+                                     const uint16_t* v, int64_t v_st, int64_t v_sh, int Nk, const int32_t* cu_k,
+                                     int32_t* status, int device, void* stream) {
+  int r = check_prefill(p);
+  if (r != 0) return r;
+  if (k == nullptr || v == nullptr || cu_k == nullptr || Nk <= 0 || Nk > (1 << 30)) return EXK_EARG;
+  if (p->N == 0) return 0;
+  DeviceScope scope;
+  if ((r = use_device(device, nullptr)) != 0) return r;
+  PrefillArgs a = {};
+  a.cu_k = cu_k;
+  a.Nk = Nk;
+  return launch_prefill(p, a, k, k_st, k_sh, v, v_st, v_sh, Nk, kTile, status, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int exk_attention_prefill_paged(const exk_prefill* p, const uint16_t* k, const uint16_t* v, int pool_pages,
+                                           const int32_t* block_table, int max_pages, const int32_t* seq_lens,
+                                           int32_t* status, int device, void* stream) {
+  int r = check_prefill(p);
+  if (r != 0) return r;
+  if (k == nullptr || v == nullptr || block_table == nullptr || seq_lens == nullptr || pool_pages <= 0 ||
+      pool_pages >= (1 << 26) || max_pages <= 0 || max_pages >= (1 << 26))
+    return EXK_EARG;
+  if (p->N == 0) return 0;
+  DeviceScope scope;
+  if ((r = use_device(device, nullptr)) != 0) return r;
+  PrefillArgs a = {};
+  a.lens = seq_lens;
+  a.block_table = block_table;
+  a.max_pages = max_pages;
+  a.pool_pages = pool_pages;
+  const int64_t st = static_cast<int64_t>(p->Hkv) * kD;
+  return launch_prefill(p, a, k, st, kD, v, st, kD, static_cast<int64_t>(pool_pages) * kP, kP, status,
+                        static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int exk_attention_prefill_paged_compressed(const exk_prefill* p, const exk_cview* k, const exk_cview* v,
+                                                      int pool_pages, const int32_t* block_table, int max_pages,
+                                                      const int32_t* seq_lens, uint16_t* k_rows, uint16_t* v_rows,
+                                                      int max_len, int32_t* status, int device, void* stream) {
+  int r = check_prefill(p);
+  if (r != 0) return r;
+  if (k == nullptr || v == nullptr || block_table == nullptr || seq_lens == nullptr || k_rows == nullptr ||
+      v_rows == nullptr || pool_pages <= 0 || pool_pages >= (1 << 26) || max_pages <= 0 || max_pages >= (1 << 26) ||
+      max_len <= 0 || max_len % kP != 0 || max_len > max_pages * kP)
+    return EXK_EARG;
+  const int64_t rows = static_cast<int64_t>(p->B) * max_len;
+  if (rows > (int64_t{1} << 30)) return EXK_EARG;
+  for (const exk_cview* c : {k, v}) {
+    if (c->sm == nullptr || c->code == nullptr || c->base == nullptr || c->rowmask == nullptr || c->rowoff == nullptr ||
+        c->raw == nullptr || c->raw_rows < 0)
+      return EXK_EARG;
+    if (!aligned16(c->sm) || !aligned16(c->code) || !aligned16(c->base) || !aligned16(c->raw)) return EXK_EALIGN;
+  }
+  if (!aligned16(k_rows) || !aligned16(v_rows)) return EXK_EALIGN;
+  if (p->N == 0) return 0;
+  DeviceScope scope;
+  if ((r = use_device(device, nullptr)) != 0) return r;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Unpack u = {};
+  u.c[0] = *k;
+  u.c[1] = *v;
+  u.out[0] = k_rows;
+  u.out[1] = v_rows;
+  u.block_table = block_table;
+  u.lens = seq_lens;
+  u.status = status;
+  u.k_stride = max_len;
+  u.B = p->B;
+  u.Hkv = p->Hkv;
+  u.max_pages = max_pages;
+  u.pool_pages = pool_pages;
+  u.pages = max_len / kP;
+  const int64_t blocks = (rows / kP * p->Hkv + 7) / 8;
+  if (blocks >= (int64_t{1} << 31)) return EXK_EARG;
+  unpack_kernel<<<dim3(static_cast<unsigned>(blocks), 2), 256, 0, st>>>(u);
+  if ((r = launch_status()) != 0) return r;
+  PrefillArgs a = {};
+  a.lens = seq_lens;
+  a.k_stride = max_len;
+  const int64_t st_e = static_cast<int64_t>(p->Hkv) * kD;
+  return launch_prefill(p, a, k_rows, st_e, kD, v_rows, st_e, kD, rows, kTile, status, st);
+}

@@ -23,7 +23,7 @@ import ctypes
 
 import torch
 
-from ._lib import CView, Partials, check, lib
+from ._lib import Append, CView, Partials, Prefill, check, lib
 
 LOG2E = 1.4426950408889634
 P = 16          # tokens per page
@@ -478,4 +478,278 @@ def attention_reference_devlen(q, k, v, T_dev, T_add=0, out=None, num_warps=None
                                        _consumer_warps(num_warps), D ** -0.5 * LOG2E,
                                        status_tensor(dev).data_ptr(), dev, stream)
     check(rc, "exk_attention_bf16_devlen")
+    return out
+
+
+# ----------------------------------------------------------------------------- new tokens into paged caches
+#
+# The paged calls below share one set of device tensors per step: block_table
+# int32 [B, max_pages], seq_lens int32 [B] (each sequence's tokens, the new
+# ones included) and, where sequences bring different numbers of new tokens,
+# cu_seqlens int32 [B + 1] (sequence b's are rows cu_seqlens[b] ..
+# cu_seqlens[b + 1] of the packed q, k, v). Rows past cu_seqlens[B] are left
+# alone, so a captured step can serve a padded batch.
+
+def rope_table(inv_freq, positions, scale=1.0):
+    """cos_sin fp32 [positions, 128] of rope_append_paged for the 64 inverse
+    frequencies inv_freq (a model's rotary_emb.inv_freq; its attention_scaling
+    as `scale`): row p holds the cosines, then the sines, of p * inv_freq. The
+    angles are formed in 64 bits."""
+    if inv_freq.shape != (D // 2,):
+        raise ValueError("inv_freq must hold 64 inverse frequencies")
+    ang = torch.arange(positions, dtype=torch.float64, device=inv_freq.device)[:, None] * inv_freq.double()
+    return (torch.cat([ang.cos(), ang.sin()], 1) * scale).float()
+
+
+def _check_rows(t, name, n, heads=None):
+    """Strided token rows [n, heads, 128] of a packed batch."""
+    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != D or t.dtype != torch.bfloat16 or not t.is_cuda or \
+            t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be a CUDA bf16 tensor [N, heads, 128] with contiguous channels")
+    st, sh = t.stride(0), t.stride(1)
+    if st % 8 or sh % 8 or t.data_ptr() % 16 or st < 0 or sh <= 0 or (st == 0 and n > 1):
+        raise ValueError(f"{name}: token and head strides must be positive multiples of 8 elements, rows 16-byte aligned")
+    return st or t.shape[1] * D, sh
+
+
+def _check_index(t, name, shape, device):
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or t.shape != shape:
+        raise ValueError(f"{name} must be a contiguous int32 tensor {list(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, slots, q_norm, k_norm, eps, q_out, Hkv, pool_pages):
+    """exk_append of a call, checked, and its output."""
+    dev = q.device
+    N, Hq, _ = q.shape if q.dim() == 3 else (0, 0, 0)
+    q_st, q_sh = _check_rows(q, "q", N)
+    k_st, k_sh = _check_rows(k, "k", N, Hkv)
+    v_st, v_sh = _check_rows(v, "v", N, Hkv)
+    if Hq % Hkv:
+        raise ValueError(f"{Hq} query heads are no multiple of {Hkv} KV heads")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [B, max_pages]")
+    B, max_pages = block_table.shape
+    if cu_seqlens is None and B != N:
+        raise ValueError("without cu_seqlens every sequence brings one token: q must be [B, heads, 128]")
+    if cos_sin.dim() != 2 or cos_sin.shape[1] != D or cos_sin.dtype != torch.float32 or cos_sin.device != dev or \
+            not cos_sin.is_contiguous():
+        raise ValueError(f"cos_sin must be a contiguous fp32 tensor [positions, 128] on {dev}")
+    if k.device != dev or v.device != dev:
+        raise ValueError("q, k and v must be on one device")
+    if (q_norm is None) != (k_norm is None):
+        raise ValueError("q_norm and k_norm come together")
+    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None and (w.dtype != torch.bfloat16 or w.shape != (D,) or w.device != dev or not w.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous bf16 tensor [128] on {dev}")
+    if q_out is None:
+        q_out = torch.empty(N, Hq, D, dtype=q.dtype, device=dev)
+    elif q_out.device != dev:
+        raise ValueError("q_out must be on q's device")
+    o_st, o_sh = _check_rows(q_out, "q_out", N, Hq)
+    a = Append(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh,
+               cos_sin.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
+               None if k_norm is None else k_norm.data_ptr(),
+               None if cu_seqlens is None else _check_index(cu_seqlens, "cu_seqlens", (B + 1,), dev),
+               _check_index(seq_lens, "seq_lens", (B,), dev),
+               _check_index(block_table, "block_table", (B, max_pages), dev),
+               None if slots is None else _check_index(slots, "slots", (B,), dev),
+               N, B, Hq, Hkv, cos_sin.shape[0], max_pages, pool_pages, eps)
+    return a, q_out
+
+
+def _bf16_pool(k, v, q):
+    """(KV heads, pages) of a pair of bf16 pools [B', TS', Hkv, 128]."""
+    for t in (k, v):
+        if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[3] != D or not t.is_contiguous() or t.shape != k.shape or \
+                t.device != q.device:
+            raise ValueError("k and v pools must be contiguous bf16 [B', TS', Hkv, 128] on q's device")
+    if k.shape[1] % P or k.numel() == 0:
+        raise ValueError("a pool's TS' must be a positive multiple of 16")
+    return k.shape[2], k.shape[0] * k.shape[1] // P
+
+
+def _coded_pool(c, q, write):
+    """(exk_cview, KV heads, pages, slots of the raw pool, counter) of a cache used as a page pool."""
+    view, TS, H = _cache_args(c)
+    if isinstance(c, dict):
+        B, sm, cap, cnt = c["shape"][0], c["sm"], c.get("cap"), c.get("cnt")
+    else:
+        B, sm, cap, cnt = c.B, c.sm, getattr(c, "cap", None), getattr(c, "cnt", None)
+    if sm.device != q.device:
+        raise ValueError("the pools must be on q's device")
+    if write and (cap is None or cnt is None):
+        raise ValueError("a pool that is written needs its raw pool's capacity (cap) and counter (cnt)")
+    return view, H, B * TS // P, cap, cnt
+
+
+def rope_append_paged(q, k, v, cos_sin, kc, vc, block_table, seq_lens, cu_seqlens=None, slots=None, q_norm=None,
+                      k_norm=None, eps=1e-6, q_out=None):
+    """Rotates a batch's new queries and keys at their positions and stores keys
+    and values in their sequences' pages of the compressed pools kc, vc (a
+    PagedCompressedKV, any CompressedKV seen as pages, or a dict of their
+    buffers with cap and cnt). q [N, Hq, 128], k, v [N, Hkv, 128] bf16, packed
+    by cu_seqlens (None: one token per sequence); channels contiguous, other
+    strides free (views of a fused projection). Sequence b's new tokens are its
+    last: positions seq_lens[b] - n_b .. seq_lens[b] - 1. cos_sin: rope_table().
+    q_norm, k_norm (bf16 [128], both or neither): RMS norm per head first.
+    Pages that fill are encoded; each sequence's last, unfilled page stays raw
+    in tail slot slots[b] (default b). The caller keeps the raw pools N * Hkv
+    rows ahead (PagedCompressedKV.ensure_headroom(N)). Returns the rotated
+    queries [N, Hq, 128] (q_out, which may be q). Positions or pages out of
+    range are not stored and reported by check_status()."""
+    kv, H, pages, k_cap, k_cnt = _coded_pool(kc, q, True)
+    vv, vH, v_pages, v_cap, v_cnt = _coded_pool(vc, q, True)
+    if vH != H or v_pages != pages:
+        raise ValueError("the key and value pools differ in shape")
+    a, q_out = _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, slots, q_norm, k_norm, eps, q_out, H,
+                            pages)
+    if a.N == 0:
+        return q_out
+    n = lib.exk_rope_append_scratch(a.N, a.B, H, cu_seqlens is not None)
+    scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
+    dev = q.device.index
+    check(lib.exk_rope_append_compressed(ctypes.byref(a), ctypes.byref(kv), k_cap, k_cnt.data_ptr(), ctypes.byref(vv),
+                                         v_cap, v_cnt.data_ptr(), scratch.data_ptr(), n,
+                                         status_tensor(dev).data_ptr(), dev,
+                                         torch.cuda.current_stream(q.device).cuda_stream), "exk_rope_append_compressed")
+    return q_out
+
+
+def rope_append_reference_paged(q, k, v, cos_sin, k_pool, v_pool, block_table, seq_lens, cu_seqlens=None, q_norm=None,
+                                k_norm=None, eps=1e-6, q_out=None):
+    """The bf16 sibling of rope_append_paged over bf16 pools [B', TS', Hkv, 128]
+    (pages of 16 rows): the same values in the same places."""
+    H, pages = _bf16_pool(k_pool, v_pool, q)
+    a, q_out = _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, None, q_norm, k_norm, eps, q_out, H,
+                            pages)
+    if a.N == 0:
+        return q_out
+    dev = q.device.index
+    check(lib.exk_rope_append_bf16(ctypes.byref(a), k_pool.data_ptr(), v_pool.data_ptr(), status_tensor(dev).data_ptr(),
+                                   dev, torch.cuda.current_stream(q.device).cuda_stream), "exk_rope_append_bf16")
+    return q_out
+
+
+# ----------------------------------------------------------------------------- prompt attention
+
+def _prefill_args(q, cu_seqlens, Hkv, max_keys, out):
+    """exk_prefill of a call, checked, its output, and the workspace it names. The
+    workspace belongs to the call (inside a capture: to the graph), so no two
+    calls share it."""
+    dev = q.device
+    N, Hq, _ = q.shape if q.dim() == 3 else (0, 0, 0)
+    q_st, q_sh = _check_rows(q, "q", N)
+    if Hq % Hkv:
+        raise ValueError(f"{Hq} query heads are no multiple of {Hkv} KV heads")
+    B = cu_seqlens.numel() - 1
+    if B < 1:
+        raise ValueError("cu_seqlens must hold B + 1 offsets")
+    cu = _check_index(cu_seqlens, "cu_seqlens", (B + 1,), dev)
+    if out is None:
+        out = torch.empty(N, Hq, D, dtype=q.dtype, device=dev)
+    elif out.device != dev:
+        raise ValueError("out must be on q's device")
+    o_st, o_sh = _check_rows(out, "out", N, Hq)
+    ns = lib.exk_prefill_splits(N, B, Hq, Hkv, max_keys, num_sms(dev.index))
+    if ns < 0:
+        check(ns, "exk_prefill_splits")
+    ws, o, m, l = None, None, None, None
+    if ns > 1:
+        rows = N * Hq * ns
+        ws = torch.empty(rows * (D + 2), dtype=torch.float32, device=dev)
+        o = ws.data_ptr()
+        m, l = o + rows * D * 4, o + rows * (D + 1) * 4
+    return Prefill(q.data_ptr(), out.data_ptr(), q_st, q_sh, o_st, o_sh, cu, o, m, l, N, B, Hq, Hkv, ns,
+                   D ** -0.5 * LOG2E), out, ws
+
+
+def attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None):
+    """Causal attention of packed prompts: q [N, Hq, 128], k, v [Nk, Hkv, 128] bf16
+    (channels contiguous, other strides free), sequence b's rows
+    cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [B + 1], device) of q and
+    cu_seqlens_k[b] .. (default cu_seqlens) of k and v. A sequence's last query
+    sees its last key, so with more keys than queries each query sees the
+    excess as context; a query that sees no key gives zeros. Up to 16 query
+    heads per KV head. Returns bf16 [N, Hq, 128]; rows past cu_seqlens[B] are
+    left as they were."""
+    if k.dim() != 3 or k.device != q.device or v.device != q.device:
+        raise ValueError("k and v must be [Nk, Hkv, 128] on q's device")
+    Nk, Hkv, _ = k.shape
+    if Nk == 0 or Hkv == 0:
+        raise ValueError("k and v must hold at least one row")
+    k_st, k_sh = _check_rows(k, "k", Nk)
+    v_st, v_sh = _check_rows(v, "v", Nk, Hkv)
+    a, out, ws = _prefill_args(q, cu_seqlens, Hkv, Nk, out)
+    if cu_seqlens_k is None:
+        if Nk != a.N:
+            raise ValueError("k and v rows differ from q's: give cu_seqlens_k")
+        cu_k = a.cu_q
+    else:
+        cu_k = _check_index(cu_seqlens_k, "cu_seqlens_k", (a.B + 1,), q.device)
+    if a.N == 0:
+        return out
+    dev = q.device.index
+    check(lib.exk_attention_prefill(ctypes.byref(a), k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, Nk, cu_k,
+                                    status_tensor(dev).data_ptr(), dev,
+                                    torch.cuda.current_stream(q.device).cuda_stream), "exk_attention_prefill")
+    return out
+
+
+def _most_keys(block_table, max_len):
+    """Keys a sequence of the call may have: max_len rounded up to whole pages, or all its pages."""
+    if block_table.dim() != 2 or block_table.shape[1] == 0:
+        raise ValueError("block_table must be [B, max_pages]")
+    cap = block_table.shape[1] * P
+    rows = cap if max_len is None else -(-max_len // P) * P
+    if not 0 < rows <= cap:
+        raise ValueError(f"max_len={max_len} out of range (1..{cap})")
+    return rows
+
+
+def _check_pages(block_table, seq_lens, B, dev):
+    max_pages = block_table.shape[1]
+    return (_check_index(block_table, "block_table", (B, max_pages), dev), max_pages,
+            _check_index(seq_lens, "seq_lens", (B,), dev))
+
+
+def attention_prefill_paged(q, kc, vc, block_table, seq_lens, cu_seqlens, max_len=None, out=None):
+    """attention_prefill with the keys and values in compressed pools (as
+    attention_paged takes them): the queries are the last tokens of sequences of
+    seq_lens[b] tokens whose pages block_table names, as rope_append_paged left
+    them. max_len (host, at least every seq_lens[b]; default max_pages * 16)
+    bounds the workspace of B * max_len decoded rows. Bit-identical to
+    attention_prefill_reference_paged for the same values and max_len."""
+    kv, H, pages, _, _ = _coded_pool(kc, q, False)
+    vv, vH, v_pages, _, _ = _coded_pool(vc, q, False)
+    if vH != H or v_pages != pages:
+        raise ValueError("the key and value pools differ in shape")
+    rows = _most_keys(block_table, max_len)
+    a, out, ws = _prefill_args(q, cu_seqlens, H, rows, out)
+    table, max_pages, lens = _check_pages(block_table, seq_lens, a.B, q.device)
+    if a.N == 0:
+        return out
+    kv_rows = torch.empty(2, a.B * rows, H, D, dtype=torch.bfloat16, device=q.device)
+    dev = q.device.index
+    check(lib.exk_attention_prefill_paged_compressed(
+        ctypes.byref(a), ctypes.byref(kv), ctypes.byref(vv), pages, table, max_pages, lens, kv_rows[0].data_ptr(),
+        kv_rows[1].data_ptr(), rows, status_tensor(dev).data_ptr(), dev,
+        torch.cuda.current_stream(q.device).cuda_stream), "exk_attention_prefill_paged_compressed")
+    return out
+
+
+def attention_prefill_reference_paged(q, k, v, block_table, seq_lens, cu_seqlens, max_len=None, out=None):
+    """The bf16 sibling of attention_prefill_paged over bf16 pools k, v [B', TS',
+    Hkv, 128] (pages of 16 rows), read in place: no workspace of rows, and max_len
+    only bounds the plan of the splits."""
+    H, pages = _bf16_pool(k, v, q)
+    a, out, ws = _prefill_args(q, cu_seqlens, H, _most_keys(block_table, max_len), out)
+    table, max_pages, lens = _check_pages(block_table, seq_lens, a.B, q.device)
+    if a.N == 0:
+        return out
+    dev = q.device.index
+    check(lib.exk_attention_prefill_paged(ctypes.byref(a), k.data_ptr(), v.data_ptr(), pages, table, max_pages, lens,
+                                          status_tensor(dev).data_ptr(), dev,
+                                          torch.cuda.current_stream(q.device).cuda_stream),
+          "exk_attention_prefill_paged")
     return out

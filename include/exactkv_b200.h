@@ -60,6 +60,7 @@ extern "C" {
 #define EXK_S_DRAIN_TIMEOUT  5  /* in-flight TMA copies did not land within 2 s */
 #define EXK_S_PEER_TIMEOUT   6  /* a peer merge waited > 2 s for another GPU's signal */
 #define EXK_S_PAGE_INDEX     7  /* a block-table entry named a page outside the pool */
+#define EXK_S_POSITION       8  /* a token's position or tail slot was out of range (not stored) */
 
 /* One compressed cache (keys or values of one layer): the six buffers of the
  * format above. raw_rows is the number of rows `raw` holds; indices at or
@@ -305,6 +306,107 @@ int exk_attention_bf16_paged(const uint16_t *q, const uint16_t *k, const uint16_
                              int B, int Hq, const int32_t *block_table, int max_pages, const int32_t *seq_lens,
                              const exk_partials *ws, uint16_t *out, int consumer_warps, float qk_scale,
                              int32_t *status, int device, void *stream);
+
+/* New tokens entering a paged cache: N packed tokens of B sequences. Sequence
+ * b's are rows [cu_seqlens[b], cu_seqlens[b+1]) of q [N, Hq, 128], k and v [N,
+ * Hkv, 128] (bf16; element strides st per token and sh per head, multiples of
+ * 8; channels contiguous; 16-byte aligned); cu_seqlens null: one token per
+ * sequence, N = B. seq_lens[b] counts the sequence's tokens with these
+ * included, so its i-th new token sits at position p = seq_lens[b] - n_b + i,
+ * in page block_table[b * max_pages + p / 16] (int32, device). cos_sin: fp32
+ * [rope_rows, 128], row p the cosines then the sines of the 64 angles of
+ * position p. Queries and keys are rotated (channel j pairs with j + 64) in
+ * fp32 with one rounding to bf16; q_norm and k_norm (bf16 [128], both or
+ * neither): each head is first scaled by weight / sqrt(mean square + eps).
+ * The rotated queries go to q_out (may be q itself). Rows at and past
+ * cu_seqlens[B] are left alone. A token whose position is outside the block
+ * table or cos_sin is not stored (in a compressed pool none of its sequence's
+ * are), its query is written as zeros, and the status word gets
+ * EXK_S_POSITION; a block-table entry outside the pool is not written
+ * (EXK_S_PAGE_INDEX). */
+typedef struct exk_append {
+  const uint16_t *q;
+  const uint16_t *k;
+  const uint16_t *v;
+  uint16_t *q_out;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;
+  const float *cos_sin;
+  const uint16_t *q_norm;
+  const uint16_t *k_norm;
+  const int32_t *cu_seqlens;
+  const int32_t *seq_lens;
+  const int32_t *block_table;
+  const int32_t *slots; /* compressed pools: tail slot of each sequence (null: b) */
+  int32_t N, B, Hq, Hkv, rope_rows, max_pages, pool_pages;
+  float eps;
+} exk_append;
+
+/* exk_append into bf16 pools [pool_pages * 16, Hkv, 128]: one launch. No
+ * counterpart in the reference (its engine rotates in PyTorch and its cache
+ * is one contiguous block). */
+int exk_rope_append_bf16(const exk_append *a, uint16_t *k_pool, uint16_t *v_pool, int32_t *status,
+                         int device, void *stream);
+
+/* exk_append into compressed pools (k, v seen as pool_pages pages of 16
+ * tokens). Pages that the call completes are encoded exactly as
+ * exk_encode_pages does, their raw rows taking slots *cnt, *cnt + 1, ... in
+ * (sequence, page, head) order; slots at or past cap are not written, so the
+ * caller keeps cap - *cnt at least N * Hkv ahead. A page left open holds its
+ * rows raw in the sequence's tail rows, raw[cap + (slots[b] * Hkv + h) * 16,
+ * + 16) (rowmask 0xFFFF), where the next call finds them. No page and no tail
+ * slot may belong to two sequences of a call that write to it. `scratch`:
+ * exk_rope_append_scratch() bytes (packed: cu_seqlens given), 16-byte
+ * aligned, in use until the call has run. Two launches. */
+int64_t exk_rope_append_scratch(int N, int B, int Hkv, int packed);
+int exk_rope_append_compressed(const exk_append *a, const exk_cview *k, int64_t k_cap, int32_t *k_cnt,
+                               const exk_cview *v, int64_t v_cap, int32_t *v_cnt, void *scratch,
+                               int64_t scratch_bytes, int32_t *status, int device, void *stream);
+
+/* Causal attention of many query tokens per sequence: N packed queries q [N,
+ * Hq, 128] (element strides q_st, q_sh, multiples of 8; 16-byte aligned),
+ * sequence b's at rows [cu_q[b], cu_q[b+1]) (int32, device), its last query at
+ * its last key: query i of n sees keys j <= i + L - n of L. A query that sees
+ * no key gives zeros; rows at and past cu_q[B] of `out` (strides o_st, o_sh)
+ * are left alone. Hq = G * Hkv, G <= 16. ns splits of each row's keys
+ * (exk_prefill_splits): with ns > 1 po [N * Hq, ns, 128], pm, pl [N * Hq, ns]
+ * fp32 hold their partials. qk_scale: log2(e) / sqrt(128). */
+typedef struct exk_prefill {
+  const uint16_t *q;
+  uint16_t *out;
+  int64_t q_st, q_sh, o_st, o_sh;
+  const int32_t *cu_q;
+  float *po;
+  float *pm;
+  float *pl;
+  int32_t N, B, Hq, Hkv, ns;
+  float qk_scale;
+} exk_prefill;
+
+/* Splits for a call of N queries of B sequences over at most max_keys keys a
+ * sequence on num_sms SMs; negative: an EXK_E* code. */
+int exk_prefill_splits(int N, int B, int Hq, int Hkv, int64_t max_keys, int num_sms);
+
+/* Keys and values packed like the queries: k, v [Nk, Hkv, 128] (strides as q),
+ * sequence b's at rows [cu_k[b], cu_k[b+1]). */
+int exk_attention_prefill(const exk_prefill *a, const uint16_t *k, int64_t k_st, int64_t k_sh,
+                          const uint16_t *v, int64_t v_st, int64_t v_sh, int Nk, const int32_t *cu_k,
+                          int32_t *status, int device, void *stream);
+
+/* Keys and values in bf16 pools [pool_pages * 16, Hkv, 128]: sequence b's
+ * first seq_lens[b] tokens (its queries' own among them) in the pages that
+ * row b of block_table [B, max_pages] names. An entry outside the pool reads
+ * as zeros (EXK_S_PAGE_INDEX). */
+int exk_attention_prefill_paged(const exk_prefill *a, const uint16_t *k, const uint16_t *v, int pool_pages,
+                                const int32_t *block_table, int max_pages, const int32_t *seq_lens,
+                                int32_t *status, int device, void *stream);
+
+/* The same over compressed pools; bit-identical for the same values. k_rows
+ * and v_rows are workspaces of [B * max_len, Hkv, 128] bf16, max_len (a
+ * multiple of 16) at least every seq_lens[b]; keys past max_len are not seen. */
+int exk_attention_prefill_paged_compressed(const exk_prefill *a, const exk_cview *k, const exk_cview *v,
+                                           int pool_pages, const int32_t *block_table, int max_pages,
+                                           const int32_t *seq_lens, uint16_t *k_rows, uint16_t *v_rows,
+                                           int max_len, int32_t *status, int device, void *stream);
 
 /* Compressed cache -> bf16 out [B, T, H, 128] through the attention kernel's
  * decoder. Replaces _dec_only_kernel/decode_to_bf16 (exactkv/kernels.py:197-211, 331-337). */
