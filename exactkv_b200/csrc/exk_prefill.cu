@@ -278,14 +278,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
 #pragma unroll
         for (int i = 0; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+        // every lane by its own row alone: a row's bits do not depend on its neighbours
+        const bool grown = top > m + kRescale;
         if (it == 0) {
           m = top;
-        } else if (__any_sync(0xFFFFFFFFu, top > m + kRescale)) {
+        } else if (__any_sync(0xFFFFFFFFu, grown)) {
           // S is complete, so the tensor core has finished O += P V of the tile before
-          const float mn = fmaxf(m, top);
-          const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
+          const float f = grown ? ex2(m - top) : 1.f;
           l *= f;
-          m = mn;
+          m = grown ? top : m;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t o[32];
