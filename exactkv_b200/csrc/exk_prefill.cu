@@ -26,7 +26,7 @@ constexpr int kTile = 128;                 // rows of a query tile, keys of a ke
 constexpr int kHalf = kTile * 128;         // bytes of one operand half: 128 rows x 64 channels bf16
 constexpr int kOperand = 2 * kHalf;        // one operand tile
 constexpr int kSlots = 4;                  // key/value ring: K, V, K, V, ...
-constexpr int kPrefillThreads = 384;       // warps 0-3, 4-7: softmax; 8: MMA; 9: TMA; 10, 11: values of masked tiles
+constexpr int kPrefillThreads = 384;       // warps 0-3, 4-7: softmax; 8: MMA; 9: TMA; 10: values of masked tiles; 11: schedule
 constexpr int kRegsSoftmax = 208, kRegsOther = 80;
 constexpr float kRescale = 8.f;            // a row's maximum may grow by 2^8 before O is rescaled
 
@@ -35,7 +35,7 @@ struct PrefillArgs {
   const int32_t* cu_k;         // packed keys, or null
   const int32_t* lens;         // keys of each sequence where cu_k is null
   const int32_t* block_table;  // pages of the keys, or null: sequence b's rows start at b * k_stride
-  int64_t k_stride;
+  int k_stride;
   const uint16_t* v;           // the values again, for non-finite ones under a mask
   int64_t v_st, v_sh;
   uint16_t* out;
@@ -67,6 +67,15 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One lane of a converged warp, the same each time. The tensor core's operands
+// are uniform registers: issued under a plain lane test, each product took
+// about 120 cycles of moves (1,050 for eight against 512 that they run).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
+}
 
 // Arrives on `bar` when every tcgen05 operation this thread issued before has completed.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
@@ -115,6 +124,36 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]),
+      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
+      : "memory");
+}
+
+// ---------------------------------------------------------------- two fp32 at once
+
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
 // Shared-memory operand descriptors, 128-byte swizzle, tiles as TMA leaves
 // them: 128-byte rows (64 channels), eight rows to a 1024-byte swizzle block.
 // K-major (Q, K: the contraction runs along the row): groups of eight rows
@@ -132,26 +171,48 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kTile / 8) << 17) | ((kTile / 16) << 24);
 constexpr uint32_t kIdescMN = kIdesc | (1u << 16);
 
-// ---------------------------------------------------------------- one CTA's work
+// ---------------------------------------------------------------- one item of work
+
+// Asks for a block of the grid that has not started: this CTA then does its
+// work in its place. The answer (16 bytes) arrives on `bar`.
+__device__ __forceinline__ void steal_block(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_addr(answer)),
+               "r"(smem_addr(bar))
+               : "memory");
+}
+// The block taken, or -1: none was left.
+__device__ __forceinline__ int stolen_block(const void* answer) {
+  int x;
+  asm volatile(
+      "{\n .reg .b128 h;\n .reg .pred p;\n ld.shared.b128 h, [%1];\n mov.b32 %0, -1;\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n}"
+      : "=r"(x)
+      : "r"(smem_addr(answer))
+      : "memory");
+  return x;
+}
 
 struct Work {
+  int valid;        // 0: no more work
+  int b, hk, split;
   int first, n;     // the sequence's first packed query, its queries
-  int L;            // its keys
-  int64_t krow;     // its first key row (not paged)
-  int b, hk;
-  int tok0;         // first token of the CTA's rows
-  int tiles;        // query tiles in use: 1 or 2
+  int L, krow;      // its keys, its first key row (not paged)
+  int tok0, tiles;  // first token of the rows; query tiles in use: 1 or 2
   int keys;         // keys that the last row sees
-  int t0, t1;       // key tiles [t0, t1) of this split
-  int low;          // keys that the first row sees (may be negative): tiles past it are masked
+  int nt, t1;       // key tiles of this split: t1 - 1 down to t1 - nt
+  int masked;       // the first of them, in which some row does not see some key
 };
 
-// Slot s of the call -> sequence and 256-row block. Sequence b's blocks take
+// Item `item` of the grid: (256-row block, KV head, split). Sequence b's blocks take
 // slots cu[b] / T + b, + 1, ... with T = 2 tpt tokens a block: n tokens need
 // at most (n + T - 1) / T, which never reaches sequence b + 1's first slot.
+// False for a slot left over. By a whole warp.
 __device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int lane, Work& w) {
   const int T = 2 * a.tpt;
-  const int split = item % a.ns;
+  if (item < 0) return false;
+  w.split = item % a.ns;
   w.hk = (item / a.ns) % a.Hkv;
   const int slot = a.slots - 1 - item / (a.ns * a.Hkv);  // long rows of keys first
   int b = 0;
@@ -160,6 +221,7 @@ __device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int la
     b += __popc(__ballot_sync(0xFFFFFFFFu, before));
   }
   if (b >= a.B) return false;
+  w.valid = 1;
   w.b = b;
   w.first = __ldg(a.cu_q + b);
   w.n = __ldg(a.cu_q + b + 1) - w.first;
@@ -168,25 +230,26 @@ __device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int la
   if (w.tok0 < 0 || w.tok0 >= w.n) return false;
   if (a.cu_k != nullptr) {
     w.krow = __ldg(a.cu_k + b);
-    w.L = __ldg(a.cu_k + b + 1) - static_cast<int>(w.krow);
-    if (w.krow < 0 || w.L < 0 || w.krow > a.Nk - w.L) w.L = 0;
+    w.L = __ldg(a.cu_k + b + 1) - w.krow;
+    if (w.krow < 0 || w.L < 0 || w.krow > a.Nk - w.L) w.L = w.krow = 0;
   } else {
     w.krow = b * a.k_stride;
     w.L = __ldg(a.lens + b);
-    const int most = a.block_table != nullptr ? a.max_pages * kP : static_cast<int>(a.k_stride);
+    const int most = a.block_table != nullptr ? a.max_pages * kP : a.k_stride;
     w.L = max(0, min(w.L, most));
   }
   w.tiles = w.n - w.tok0 > a.tpt ? 2 : 1;
-  w.low = w.L - w.n + w.tok0 + 1;
   w.keys = max(0, w.L - w.n + min(w.tok0 + T, w.n));
-  const int nt = (w.keys + kTile - 1) / kTile;
-  const int per = (nt + a.ns - 1) / a.ns;
-  w.t0 = min(nt, split * per);
-  w.t1 = min(nt, w.t0 + per);
+  const int all = (w.keys + kTile - 1) / kTile;
+  const int per = (all + a.ns - 1) / a.ns;
+  const int t0 = min(all, w.split * per);
+  w.t1 = min(all, t0 + per);
+  w.nt = w.t1 - t0;
+  // tile j holds a key past the first row's last one when (j + 1) * 128 > low
+  const int low = w.L - w.n + w.tok0 + 1;
+  w.masked = min(w.nt, max(0, w.t1 - max(0, low) / kTile));
   return true;
 }
-
-__device__ __forceinline__ bool tile_masked(const Work& w, int j) { return (j + 1) * kTile > w.low; }
 
 // Waits that end: after kWaitLimitNs, or at once when another role gave up.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
@@ -207,14 +270,154 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, stop));
 }
 
-struct __align__(8) Bars {
-  uint64_t q_full[2], kv_full[kSlots], kv_empty[kSlots], v_ok[kSlots], s_full[2], p_full[2], o_full[2];
+struct __align__(16) Bars {
+  uint4 answer;
+  uint64_t q_full[2], q_empty[2], kv_full[kSlots], kv_empty[kSlots], v_ok[kSlots], s_full[2], p_full[2], o_full[2];
+  uint64_t work_full[2], work_empty[2], block, want;
+  Work work[2];
   uint32_t tmem;
   int stop, bad;
 };
 
 constexpr int kPrefillSmem = 2 * kOperand + kSlots * kOperand + static_cast<int>(sizeof(Bars)) + 1024;
 
+// The softmax threads' side of one item: query tile x, a row per thread. s_phase:
+// tiles of S this thread has taken so far.
+__device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w, Bars* bars, uint32_t tmem, int x,
+                                             uint32_t& s_phase, uint32_t& o_phase, volatile int* stop) {
+  const int warp = threadIdx.x >> 5, r = threadIdx.x & 127;
+  const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+  const uint32_t ts = tmem + lanes + x * kTile, to = tmem + lanes + 2 * kTile + x * kTile;
+  const int tok = w.tok0 + x * a.tpt + r / a.G;
+  const bool valid = r < a.G * a.tpt && tok < w.n;
+  const int lim = valid ? w.L - w.n + tok : -1;  // last key the row sees
+  const int nt = w.nt;
+  float m = -INFINITY, l = 0.f;
+  for (int it = 0; it < nt; ++it) {
+    if (!warp_wait(&bars->s_full[x], s_phase & 1, stop)) break;
+    ++s_phase;
+    tc_fence_after();
+    uint32_t s[kTile];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
+    tc_wait_ld();
+    if (it < w.masked) {
+      const int seen = lim - (w.t1 - 1 - it) * kTile;
+#pragma unroll
+      for (int i = 0; i < kTile; ++i)
+        if (i > seen) s[i] = 0xFF800000u;
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+    // The maximum follows by steps of 2^kRescale at least: P stays below
+    // 2^kRescale, and O is rarely rescaled. Every lane decides by its own row
+    // alone, so a row's bits do not depend on its neighbours.
+    const bool grown = valid && top > m + kRescale;
+    if (it == 0) {
+      m = top;
+    } else if (__any_sync(0xFFFFFFFFu, grown)) {
+      // S is complete, so the tensor core has finished O += P V of the tile before
+      const float f = grown ? ex2(m - top) : 1.f;
+      l *= f;
+      m = grown ? top : m;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        tmem_ld32(to + 32 * c, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tmem_st32(to + 32 * c, o);
+      }
+    }
+    const float off = m == -INFINITY ? 0.f : -m;
+    const F2 scale2 = f2(a.scale, a.scale), off2 = f2(off, off);
+    F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int e = 32 * c + 2 * i;
+        float p0, p1;
+        split2(fma2(f2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, off2), p0, p1);
+        p0 = ex2(p0);
+        p1 = ex2(p1);
+        sum[i & 1] = add2(sum[i & 1], f2(p0, p1));
+        p[i] = pack_bf16x2(p0, p1);
+      }
+      tmem_st16(ts + 16 * c, p);
+    }
+    float l0, l1;
+    split2(add2(sum[0], sum[1]), l0, l1);
+    l += l0 + l1;
+    tc_wait_st();
+    tc_fence_before();
+    mbar_arrive(&bars->p_full[x]);
+  }
+  bool have = false;
+  if (nt > 0) {
+    have = warp_wait(&bars->o_full[x], o_phase & 1, stop);
+    ++o_phase;
+    tc_fence_after();
+  }
+  const int h = w.hk * a.G + r % a.G;
+  const int64_t row = static_cast<int64_t>(w.first + tok) * a.Hq + h;
+  if (a.ns > 1 && valid) {
+    a.pm[row * a.ns + w.split] = have ? m : -INFINITY;
+    a.pl[row * a.ns + w.split] = have ? l : 0.f;
+  }
+  const float inv = a.ns > 1 ? 1.f : (have && l > 0.f ? 1.f / l : (l != l ? l : 0.f));
+  const bool bad = *const_cast<volatile int*>(&bars->bad) != 0;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t o[32];
+    if (have) {
+      tmem_ld32(to + 32 * c, o);
+      tc_wait_ld();
+    }
+    if (!valid) continue;
+    float f[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = have && !(l == 0.f) ? __uint_as_float(o[i]) * inv : 0.f;
+    if (bad) {
+      // a masked tile held values that are not finite: they were left out of
+      // the product and reach the rows that see them here
+      for (int t = (w.t1 - w.masked) * kTile; t < min(w.t1 * kTile, lim + 1); ++t) {
+        int64_t vrow = static_cast<int64_t>(w.krow) + t;
+        if (a.block_table != nullptr) {
+          const int pg = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + t / kP);
+          if (pg < 0 || pg >= a.pool_pages) continue;
+          vrow = static_cast<int64_t>(pg) * kP + t % kP;
+        }
+        const uint16_t* vp = a.v + vrow * a.v_st + w.hk * a.v_sh + 32 * c;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if ((vp[i] & 0x7F80) == 0x7F80) f[i] += __uint_as_float(static_cast<uint32_t>(vp[i]) << 16);
+      }
+    }
+    if (a.ns > 1) {
+      float4* d = reinterpret_cast<float4*>(a.po + (row * a.ns + w.split) * kD + 32 * c);
+      if (have) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+      }
+    } else {
+      uint4* d = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(w.first + tok) * a.o_st + h * a.o_sh + 32 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        d[i] = make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
+                          pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+    }
+  }
+  tc_fence_before();
+}
+
+// One CTA per SM, which takes blocks of the grid as they come (longest first):
+// while one item's rows are written out, the next one's operands are loaded and
+// its first S is computed.
 __global__ void __launch_bounds__(kPrefillThreads, 1)
     prefill_kernel(const __grid_constant__ PrefillArgs a, const __grid_constant__ PrefillMaps maps) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -222,23 +425,26 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   uint8_t* sq = smem;
   uint8_t* ring = smem + 2 * kOperand;
   Bars* bars = reinterpret_cast<Bars*>(ring + kSlots * kOperand);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* stop = &bars->stop;
 
-  Work w;
-  if (!load_work(a, blockIdx.x, lane, w)) return;  // the whole CTA
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->q_empty[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], kTile);
       mbar_init(&bars->o_full[i], 1);
+      mbar_init(&bars->work_full[i], 1);
+      mbar_init(&bars->work_empty[i], 11);
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&bars->kv_full[i], 1);
-      mbar_init(&bars->kv_empty[i], 1);
-      mbar_init(&bars->v_ok[i], 64);
+      mbar_init(&bars->kv_empty[i], 1 + (i & 1));  // V entries (odd): the products and warp 10
+      mbar_init(&bars->v_ok[i], 32);
     }
+    mbar_init(&bars->block, 1);
+    mbar_init(&bars->want, 1);
     bars->stop = bars->bad = 0;
     fence_mbar_init();
   }
@@ -247,264 +453,232 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
-  const int nt = w.t1 - w.t0;  // key tiles, from w.t1 - 1 down
+  // Work number `k` of this CTA, as the scheduling warp left it: false at the end.
+  uint32_t k = 0;
+  auto next_work = [&](Work& w) {
+    const int i = k & 1;
+    const bool ok = warp_wait(&bars->work_full[i], (k >> 1) & 1, stop);
+    w = bars->work[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->work_empty[i]);
+    ++k;
+    return ok && w.valid != 0;
+  };
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    const int x = warp >> 2;                 // query tile
-    const int r = threadIdx.x & 127;         // row
-    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
-    const uint32_t ts = tmem + lanes + x * kTile, to = tmem + lanes + 2 * kTile + x * kTile;
-    const int tok = w.tok0 + x * a.tpt + r / a.G;
-    const bool valid = r < a.G * a.tpt && tok < w.n;
-    const int lim = w.L - w.n + tok;         // last key the row sees
-    float m = -INFINITY, l = 0.f;
-    if (x < w.tiles) {
-      for (int it = 0; it < nt; ++it) {
-        const int j = w.t1 - 1 - it;
-        if (!warp_wait(&bars->s_full[x], it & 1, stop)) break;
-        tc_fence_after();
-        uint32_t s[kTile];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
-        tc_wait_ld();
-        if (tile_masked(w, j)) {
-          const int seen = lim - j * kTile;
-#pragma unroll
-          for (int i = 0; i < kTile; ++i)
-            if (i > seen) s[i] = 0xFF800000u;
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
-        // every lane by its own row alone: a row's bits do not depend on its neighbours
-        const bool grown = top > m + kRescale;
-        if (it == 0) {
-          m = top;
-        } else if (__any_sync(0xFFFFFFFFu, grown)) {
-          // S is complete, so the tensor core has finished O += P V of the tile before
-          const float f = grown ? ex2(m - top) : 1.f;
-          l *= f;
-          m = grown ? top : m;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld32(to + 32 * c, o);
-            tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st32(to + 32 * c, o);
-          }
-        }
-        const float off = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t p[kTile / 2];
-#pragma unroll
-        for (int i = 0; i < kTile; i += 2) {
-          const float p0 = ex2(fmaf(__uint_as_float(s[i]), a.scale, off));
-          const float p1 = ex2(fmaf(__uint_as_float(s[i + 1]), a.scale, off));
-          sum[(i >> 1) & 3] += p0 + p1;
-          p[i >> 1] = pack_bf16x2(p0, p1);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st32(ts, p);
-        tmem_st32(ts + 32, p + 32);
-        tc_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bars->p_full[x]);
-      }
-      const bool have = nt > 0 && warp_wait(&bars->o_full[x], 0, stop);
-      tc_fence_after();
-      const int h = w.hk * a.G + r % a.G;
-      const int64_t row = static_cast<int64_t>(w.first + tok) * a.Hq + h;
-      if (a.ns > 1 && valid) {
-        const int split = blockIdx.x % a.ns;
-        a.pm[row * a.ns + split] = have ? m : -INFINITY;
-        a.pl[row * a.ns + split] = have ? l : 0.f;
-      }
-      const float inv = a.ns > 1 ? 1.f : (have && l > 0.f ? 1.f / l : (l != l ? l : 0.f));
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
-        if (have) {
-          tmem_ld32(to + 32 * c, o);
-          tc_wait_ld();
-        }
-        if (!valid) continue;
-        float f[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = have && !(l == 0.f) ? __uint_as_float(o[i]) * inv : 0.f;
-        if (bars->bad != 0) {
-          // a masked tile held values that are not finite: they were left out of
-          // the product and reach the rows that see them here
-          for (int j = w.t0; j < w.t1; ++j) {
-            if (!tile_masked(w, j)) continue;
-            for (int t = j * kTile; t < min((j + 1) * kTile, lim + 1); ++t) {
-              int64_t vrow = w.krow + t;
-              if (a.block_table != nullptr) {
-                const int pg = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + t / kP);
-                if (pg < 0 || pg >= a.pool_pages) continue;
-                vrow = static_cast<int64_t>(pg) * kP + t % kP;
-              }
-              const uint16_t* vp = a.v + vrow * a.v_st + w.hk * a.v_sh + 32 * c;
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if ((vp[i] & 0x7F80) == 0x7F80) f[i] += __uint_as_float(static_cast<uint32_t>(vp[i]) << 16);
-            }
-          }
-        }
-        if (a.ns > 1) {
-          float4* d = reinterpret_cast<float4*>(a.po + (row * a.ns + blockIdx.x % a.ns) * kD + 32 * c);
-          if (have) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-          }
-        } else {
-          uint4* d = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(w.first + tok) * a.o_st + h * a.o_sh + 32 * c);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            d[i] = make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
-                              pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
-        }
-      }
-    }
-    tc_fence_before();
+    const int x = warp >> 2;
+    uint32_t s_phase = 0, o_phase = 0;
+    Work w;
+    while (next_work(w))
+      if (x < w.tiles) softmax_item(a, w, bars, tmem, x, s_phase, o_phase, stop);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == 8 && nt > 0) {
-      // ---- MMA: K of tile `it` is ring entry 2 it, V is 2 it + 1
-      auto qk = [&](int x, int slot) {
-        if (lane == 0) {
-          const uint32_t qa = smem_addr(sq) + x * kOperand, ka = smem_addr(ring) + slot * kOperand;
+    if (warp == 8) {
+      // ---- MMA: K of an item's tile `it` is ring entry e + 2 it, V the one after
+      const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+      const uint64_t dq = desc_kmajor(smem_addr(sq)), dk = desc_kmajor(smem_addr(ring)), dv = desc_mnmajor(smem_addr(ring));
+      uint32_t e = 0, q_phase = 0, p_phase = 0, ok_phase = 0;  // bit x (or slot): the parity to wait for next
+      // S of query tile x from the K in `slot`; `last`: the item's last use of Q
+      auto qk = [&](int x, uint32_t slot, bool last) {
+        if (elect_one()) {
+          const uint64_t a0 = dq + x * (kOperand >> 4), b0 = dk + slot * (kOperand >> 4);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
-            mma_ss(tmem + x * kTile, desc_kmajor(qa + off), desc_kmajor(ka + off), kIdesc, k > 0);
+          for (int c = 0; c < 8; ++c) {
+            const uint64_t off = ((c >> 2) * kHalf + (c & 3) * 32) >> 4;
+            mma_ss(tm + x * kTile, a0 + off, b0 + off, kIdesc, c > 0);
           }
           tc_commit(&bars->s_full[x]);
+          if (last) tc_commit(&bars->q_empty[x]);
         }
         __syncwarp();
       };
-      bool ok = true;
-      for (int x = 0; x < w.tiles && ok; ++x) {
-        ok = warp_wait(&bars->q_full[x], 0, stop) && (x > 0 || warp_wait(&bars->kv_full[0], 0, stop));
-        tc_fence_after();
-        if (ok) qk(x, 0);
-      }
-      if (ok && lane == 0) tc_commit(&bars->kv_empty[0]);
-      for (int it = 0; it < nt && ok; ++it) {
-        const int ve = 2 * it + 1, ke = 2 * it + 2;
-        const int vs = ve % kSlots, ks = ke % kSlots;
-        const uint32_t vph = (ve / kSlots) & 1, kph = (ke / kSlots) & 1;
-        for (int x = 0; x < w.tiles && ok; ++x) {
-          if (x == 0) {
-            // the masked tiles come first, so the k-th use of v_ok[vs] is the k-th use of the slot
-            ok = warp_wait(tile_masked(w, w.t1 - 1 - it) ? &bars->v_ok[vs] : &bars->kv_full[vs], vph, stop);
-          }
-          ok = ok && warp_wait(&bars->p_full[x], it & 1, stop);
-          if (!ok) break;
+      Work w;
+      while (next_work(w)) {
+        const int nt = __shfl_sync(0xFFFFFFFFu, w.nt, 0), tiles = __shfl_sync(0xFFFFFFFFu, w.tiles, 0);
+        const int masked = __shfl_sync(0xFFFFFFFFu, w.masked, 0);
+        if (nt == 0) continue;
+        bool ok = warp_wait(&bars->kv_full[e % kSlots], (e / kSlots) & 1, stop);
+        for (int x = 0; x < tiles && ok; ++x) {
+          ok = warp_wait(&bars->q_full[x], (q_phase >> x) & 1, stop);
+          q_phase ^= 1u << x;
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t va = smem_addr(ring) + vs * kOperand;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              mma_ts(tmem + 2 * kTile + x * kTile, tmem + x * kTile + 8 * k, desc_mnmajor(va + 2048 * k), kIdescMN,
-                     it > 0 || k > 0);
-            if (x == w.tiles - 1) tc_commit(&bars->kv_empty[vs]);
-            if (it == nt - 1) tc_commit(&bars->o_full[x]);
-          }
-          __syncwarp();
-          if (it < nt - 1) {
-            if (x == 0) ok = warp_wait(&bars->kv_full[ks], kph, stop);
-            if (ok) qk(x, ks);
-          }
+          if (ok) qk(x, e % kSlots, nt == 1);
         }
-        if (ok && it < nt - 1 && lane == 0) tc_commit(&bars->kv_empty[ks]);
+        if (ok && elect_one()) tc_commit(&bars->kv_empty[e % kSlots]);
+        for (int it = 0; it < nt && ok; ++it) {
+          const uint32_t ve = e + 2 * it + 1, ke = ve + 1, vs = ve % kSlots, ks = ke % kSlots;
+          if (it < masked) {
+            ok = warp_wait(&bars->v_ok[vs], (ok_phase >> vs) & 1, stop);
+            ok_phase ^= 1u << vs;
+          } else {
+            ok = warp_wait(&bars->kv_full[vs], (ve / kSlots) & 1, stop);
+          }
+          for (int x = 0; x < tiles && ok; ++x) {
+            ok = warp_wait(&bars->p_full[x], (p_phase >> x) & 1, stop);
+            p_phase ^= 1u << x;
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t b0 = dv + vs * (kOperand >> 4);
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                mma_ts(tm + 2 * kTile + x * kTile, tm + x * kTile + 8 * c, b0 + c * (2048 >> 4), kIdescMN, it > 0 || c > 0);
+              if (x == tiles - 1) tc_commit(&bars->kv_empty[vs]);
+              if (it == nt - 1) tc_commit(&bars->o_full[x]);
+            }
+            __syncwarp();
+            if (it < nt - 1) {
+              if (x == 0) ok = warp_wait(&bars->kv_full[ks], (ke / kSlots) & 1, stop);
+              if (ok) qk(x, ks, it == nt - 2);
+            }
+          }
+          if (ok && it < nt - 1 && elect_one()) tc_commit(&bars->kv_empty[ks]);
+        }
+        e += 2 * nt;
+        if (!ok) break;
       }
-    } else if (warp == 9 && nt > 0) {
+    } else if (warp == 9) {
       // ---- TMA
       const int tile_bytes = 64 * 2 * a.G * a.tpt;
+      uint32_t e = 0, q_phase = 3;
       if (lane == 0) {
         prefetch_tmap(&maps.q);
         prefetch_tmap(&maps.k);
         prefetch_tmap(&maps.v);
-        for (int x = 0; x < w.tiles; ++x) {
-          mbar_arrive_expect_tx(&bars->q_full[x], 2 * tile_bytes);
-          for (int c = 0; c < 2; ++c)
-            tma_load_3d(sq + x * kOperand + c * kHalf, &maps.q, 64 * c, w.hk * a.G, w.first + w.tok0 + x * a.tpt,
-                        &bars->q_full[x]);
-        }
       }
-      for (int e = 0; e < 2 * nt; ++e) {
-        const int slot = e % kSlots, j = w.t1 - 1 - e / 2;
-        if (e >= kSlots && !warp_wait(&bars->kv_empty[slot], ((e / kSlots) & 1) ^ 1, stop)) break;
-        const CUtensorMap* map = (e & 1) == 0 ? &maps.k : &maps.v;
-        uint8_t* dst = ring + slot * kOperand;
-        if (a.block_table == nullptr) {
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars->kv_full[slot], kOperand);
+      Work w;
+      while (next_work(w)) {
+        bool ok = true;
+        for (int x = 0; w.nt > 0 && x < w.tiles && ok; ++x) {
+          ok = warp_wait(&bars->q_empty[x], (q_phase >> x) & 1, stop);
+          q_phase ^= 1u << x;
+          if (ok && lane == 0) {
+            mbar_arrive_expect_tx(&bars->q_full[x], 2 * tile_bytes);
             for (int c = 0; c < 2; ++c)
-              tma_load_3d(dst + c * kHalf, map, 64 * c, w.hk, static_cast<int>(w.krow) + j * kTile, &bars->kv_full[slot]);
+              tma_load_3d(sq + x * kOperand + c * kHalf, &maps.q, 64 * c, w.hk * a.G, w.first + w.tok0 + x * a.tpt,
+                          &bars->q_full[x]);
           }
-        } else {
-          // one lane per page; pages past the keys are not loaded (their columns are masked)
-          const int pages = min(kTile / kP, (w.keys - j * kTile + kP - 1) / kP);
-          int row = 0;
-          if (lane < pages) {
-            const int pg = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + j * (kTile / kP) + lane);
-            if (pg >= 0 && pg < a.pool_pages) {
-              row = pg * kP;
-            } else {
-              set_status(a.status, EXK_S_PAGE_INDEX);
-              row = a.pool_pages * kP;  // outside the map: zeros
+        }
+        for (int i = 0; i < 2 * w.nt && ok; ++i, ++e) {
+          const uint32_t slot = e % kSlots;
+          const int j = w.t1 - 1 - i / 2;
+          ok = warp_wait(&bars->kv_empty[slot], ((e / kSlots) & 1) ^ 1, stop);
+          if (!ok) break;
+          const CUtensorMap* map = (i & 1) == 0 ? &maps.k : &maps.v;
+          uint8_t* dst = ring + slot * kOperand;
+          if (a.block_table == nullptr) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&bars->kv_full[slot], kOperand);
+              for (int c = 0; c < 2; ++c)
+                tma_load_3d(dst + c * kHalf, map, 64 * c, w.hk, w.krow + j * kTile, &bars->kv_full[slot]);
+            }
+          } else {
+            // one lane per page; pages past the keys are not loaded (their columns are masked)
+            const int pages = min(kTile / kP, (w.keys - j * kTile + kP - 1) / kP);
+            int row = 0;
+            if (lane < pages) {
+              const int pg = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + j * (kTile / kP) + lane);
+              if (pg >= 0 && pg < a.pool_pages) {
+                row = pg * kP;
+              } else {
+                set_status(a.status, EXK_S_PAGE_INDEX);
+                row = a.pool_pages * kP;  // outside the map: zeros
+              }
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[slot], pages * (2 * 64 * 2 * kP));
+            __syncwarp();
+            if (lane < pages) {
+              for (int c = 0; c < 2; ++c)
+                tma_load_3d(dst + c * kHalf + lane * (kP * 128), map, 64 * c, w.hk, row, &bars->kv_full[slot]);
             }
           }
-          if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[slot], pages * (2 * 64 * 2 * kP));
           __syncwarp();
-          if (lane < pages) {
-            for (int c = 0; c < 2; ++c)
-              tma_load_3d(dst + c * kHalf + lane * (kP * 128), map, 64 * c, w.hk, row, &bars->kv_full[slot]);
-          }
         }
-        __syncwarp();
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(&bars->want);
       }
-    } else if (warp >= 10 && nt > 0) {
+    } else if (warp == 10) {
       // ---- values of masked tiles: rows past the last key become zeros, and so do
       // values that are not finite (0 x inf would reach rows that do not see them)
-      for (int it = 0; it < nt && tile_masked(w, w.t1 - 1 - it); ++it) {
-        const int j = w.t1 - 1 - it, ve = 2 * it + 1, vs = ve % kSlots;
-        if (!bar_wait(&bars->kv_full[vs], (ve / kSlots) & 1, stop)) break;
-        const int t = threadIdx.x - 320;
-        uint4* v = reinterpret_cast<uint4*>(ring + vs * kOperand);
-        bool bad = false;
-        const int rows = w.keys - j * kTile;  // keys of the tile that some row sees
-        for (int i = t; i < kOperand / 16; i += 64) {
-          const int row = (i >> 3) & (kTile - 1);
-          if (row >= rows) {
-            v[i] = make_uint4(0, 0, 0, 0);
-          } else {
-            uint4 u = v[i];
-            uint32_t e[4] = {u.x, u.y, u.z, u.w};
-            bool hit = false;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if ((e[k] & 0x7F80u) == 0x7F80u) {
-                e[k] &= 0xFFFF0000u;
-                hit = true;
-              }
-              if ((e[k] & 0x7F800000u) == 0x7F800000u) {
-                e[k] &= 0xFFFFu;
-                hit = true;
+      uint32_t e = 0;
+      Work w;
+      while (next_work(w)) {
+        bool ok = true;
+        for (int it = 0; it < w.nt && ok; ++it) {
+          // (every tile, and the ring waits for this warp: a wait on a phase of a
+          // barrier that may be two phases ahead or behind would not be one)
+          const uint32_t ve = e + 2 * it + 1, vs = ve % kSlots;
+          ok = warp_wait(&bars->kv_full[vs], (ve / kSlots) & 1, stop);
+          if (!ok) break;
+          if (it >= w.masked) {
+            if (lane == 0) mbar_arrive(&bars->kv_empty[vs]);
+            continue;
+          }
+          uint4* v = reinterpret_cast<uint4*>(ring + vs * kOperand);
+          bool bad = false;
+          const int rows = w.keys - (w.t1 - 1 - it) * kTile;  // keys of the tile that some row sees
+#pragma unroll 4
+          for (int i = lane; i < kOperand / 16; i += 32) {
+            const int row = (i >> 3) & (kTile - 1);
+            if (row >= rows) {
+              v[i] = make_uint4(0, 0, 0, 0);
+            } else {
+              // bit 15 of each half: exponent field all ones
+              uint4 u = v[i];
+              const uint32_t b0 = ((u.x & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+              const uint32_t b1 = ((u.y & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+              const uint32_t b2 = ((u.z & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+              const uint32_t b3 = ((u.w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+              if ((b0 | b1 | b2 | b3) != 0u) {
+                u.x &= ~((b0 >> 15) * 0xFFFFu);
+                u.y &= ~((b1 >> 15) * 0xFFFFu);
+                u.z &= ~((b2 >> 15) * 0xFFFFu);
+                u.w &= ~((b3 >> 15) * 0xFFFFu);
+                v[i] = u;
+                bad = true;
               }
             }
-            if (hit) v[i] = make_uint4(e[0], e[1], e[2], e[3]);
-            bad |= hit;
           }
+          // (kept for the CTA's later items: they then look for such values too)
+          if (bad) *const_cast<volatile int*>(&bars->bad) = 1;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(&bars->v_ok[vs]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->kv_empty[vs]);
         }
-        if (bad) *const_cast<volatile int*>(&bars->bad) = 1;
+        e += 2 * w.nt;
+        if (!ok) break;
+      }
+    } else {
+      // ---- schedule: this CTA's own block, then blocks that have not started. The
+      // next is asked for when the last copies of an item are under way, about two
+      // key tiles before it ends: asked for sooner, a CTA with a long item would hold
+      // back another that an idle one could start (4096 tokens: 174 us for 150).
+      int item = blockIdx.x;
+      uint32_t asked = 0, wanted = 0;
+      Work w;
+      while (true) {
+        const bool some = load_work(a, item, lane, w);
+        if (!some) w.valid = 0;
+        if (some || item < 0) {
+          if (!warp_wait(&bars->work_empty[k & 1], ((k >> 1) & 1) ^ 1, stop)) break;
+          if (lane == 0) {
+            bars->work[k & 1] = w;
+            mbar_arrive(&bars->work_full[k & 1]);
+          }
+          ++k;
+          if (item < 0) break;
+          if (!warp_wait(&bars->want, wanted++ & 1, stop)) break;
+        }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->block, 16);
+          steal_block(&bars->answer, &bars->block);
+        }
+        if (!warp_wait(&bars->block, asked++ & 1, stop)) break;
+        item = stolen_block(&bars->answer);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&bars->v_ok[vs]);
+        __syncwarp();
       }
     }
   }
