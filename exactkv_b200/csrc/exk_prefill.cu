@@ -154,6 +154,12 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Shared-memory operand descriptors, 128-byte swizzle, tiles as TMA leaves
 // them: 128-byte rows (64 channels), eight rows to a 1024-byte swizzle block.
 // K-major (Q, K: the contraction runs along the row): groups of eight rows
@@ -272,18 +278,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 
 struct __align__(16) Bars {
   uint4 answer;
-  uint64_t q_full[2], q_empty[2], kv_full[kSlots], kv_empty[kSlots], v_ok[kSlots], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], q_empty[2], kv_full[kSlots], kv_empty[kSlots], v_ok[kSlots], s_full[2], p_most[2], p_full[2], o_full[2];
   uint64_t work_full[2], work_empty[2], block, want;
   Work work[2];
   uint32_t tmem;
   int stop, bad;
 };
 
-constexpr int kPrefillSmem = 2 * kOperand + kSlots * kOperand + static_cast<int>(sizeof(Bars)) + 1024;
+constexpr int kStage = 8 * 32 * 128;
+constexpr int kPrefillSmem = 2 * kOperand + kSlots * kOperand + kStage + static_cast<int>(sizeof(Bars)) + 1024;
 
 // The softmax threads' side of one item: query tile x, a row per thread. s_phase:
 // tiles of S this thread has taken so far.
-__device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w, Bars* bars, uint32_t tmem, int x,
+__device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w, Bars* bars, uint4* stage, uint32_t tmem, int x,
                                              uint32_t& s_phase, uint32_t& o_phase, volatile int* stop) {
   const int warp = threadIdx.x >> 5, r = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
@@ -309,8 +316,9 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
     }
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
-    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale;
+    for (int i = 0; i < kTile; i += 2)
+      mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+    const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale;
     // The maximum follows by steps of 2^kRescale at least: P stays below
     // 2^kRescale, and O is rarely rescaled. Every lane decides by its own row
     // alone, so a row's bits do not depend on its neighbours.
@@ -349,6 +357,11 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
         p[i] = pack_bf16x2(p0, p1);
       }
       tmem_st16(ts + 16 * c, p);
+      if (c == 2) {  // three quarters: the product may start
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars->p_most[x]);
+      }
     }
     float l0, l1;
     split2(add2(sum[0], sum[1]), l0, l1);
@@ -371,6 +384,27 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
   }
   const float inv = a.ns > 1 ? 1.f : (have && l > 0.f ? 1.f / l : (l != l ? l : 0.f));
   const bool bad = *const_cast<volatile int*>(&bars->bad) != 0;
+  // The row's place; null: not written (no row, or a split without keys).
+  uint64_t dst = 0;
+  if (valid && a.ns == 1)
+    dst = reinterpret_cast<uint64_t>(a.out + static_cast<int64_t>(w.first + tok) * a.o_st + h * a.o_sh);
+  if (valid && a.ns > 1 && have) dst = reinterpret_cast<uint64_t>(a.po + (row * a.ns + w.split) * kD);
+  // 128 bytes of every row at a time go through shared memory, 16-byte pieces
+  // swizzled by row, so that eight lanes write a whole line: stored by the rows'
+  // own threads, 16 bytes a row, the tile took 6,000 cycles.
+  uint4* mine = stage + warp * 256;
+  const int lane = threadIdx.x & 31;
+  auto flush = [&](int part) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int from = 4 * i + (lane >> 3);
+      const uint64_t d = __shfl_sync(0xFFFFFFFFu, dst, from);
+      const uint4 v = mine[from * 8 + ((lane & 7) ^ (from & 7))];
+      if (d != 0) reinterpret_cast<uint4*>(d + 128 * part)[lane & 7] = v;
+    }
+    __syncwarp();
+  };
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     uint32_t o[32];
@@ -378,11 +412,10 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
       tmem_ld32(to + 32 * c, o);
       tc_wait_ld();
     }
-    if (!valid) continue;
     float f[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] = have && !(l == 0.f) ? __uint_as_float(o[i]) * inv : 0.f;
-    if (bad) {
+    if (bad && valid) {
       // a masked tile held values that are not finite: they were left out of
       // the product and reach the rows that see them here
       for (int t = (w.t1 - w.masked) * kTile; t < min(w.t1 * kTile, lim + 1); ++t) {
@@ -399,17 +432,18 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
       }
     }
     if (a.ns > 1) {
-      float4* d = reinterpret_cast<float4*>(a.po + (row * a.ns + w.split) * kD + 32 * c);
-      if (have) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-      }
+      for (int i = 0; i < 8; ++i)
+        mine[lane * 8 + (i ^ (lane & 7))] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]),
+                                                       __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+      flush(c);
     } else {
-      uint4* d = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(w.first + tok) * a.o_st + h * a.o_sh + 32 * c);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        d[i] = make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
-                          pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+        mine[lane * 8 + ((4 * (c & 1) + i) ^ (lane & 7))] =
+            make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
+                       pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+      if (c & 1) flush(c >> 1);
     }
   }
   tc_fence_before();
@@ -424,7 +458,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   uint8_t* sq = smem;
   uint8_t* ring = smem + 2 * kOperand;
-  Bars* bars = reinterpret_cast<Bars*>(ring + kSlots * kOperand);
+  uint4* stage = reinterpret_cast<uint4*>(ring + kSlots * kOperand);  // 32 rows of 128 bytes for each softmax warp
+  Bars* bars = reinterpret_cast<Bars*>(ring + kSlots * kOperand + kStage);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* stop = &bars->stop;
 
@@ -433,6 +468,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       mbar_init(&bars->q_full[i], 1);
       mbar_init(&bars->q_empty[i], 1);
       mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_most[i], kTile);
       mbar_init(&bars->p_full[i], kTile);
       mbar_init(&bars->o_full[i], 1);
       mbar_init(&bars->work_full[i], 1);
@@ -471,7 +507,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     uint32_t s_phase = 0, o_phase = 0;
     Work w;
     while (next_work(w))
-      if (x < w.tiles) softmax_item(a, w, bars, tmem, x, s_phase, o_phase, stop);
+      if (x < w.tiles) softmax_item(a, w, bars, stage, tmem, x, s_phase, o_phase, stop);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == 8) {
@@ -515,15 +551,25 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             ok = warp_wait(&bars->kv_full[vs], (ve / kSlots) & 1, stop);
           }
           for (int x = 0; x < tiles && ok; ++x) {
+            // P comes in two parts, 96 keys and 32: the first part's product runs
+            // beside the last exponentials
+            const uint64_t b0 = dv + vs * (kOperand >> 4);
+            const uint32_t d = tm + 2 * kTile + x * kTile, p0 = tm + x * kTile;
+            ok = warp_wait(&bars->p_most[x], (p_phase >> x) & 1, stop);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int c = 0; c < 6; ++c) mma_ts(d, p0 + 8 * c, b0 + c * (2048 >> 4), kIdescMN, it > 0 || c > 0);
+            }
+            __syncwarp();
             ok = warp_wait(&bars->p_full[x], (p_phase >> x) & 1, stop);
             p_phase ^= 1u << x;
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
-              const uint64_t b0 = dv + vs * (kOperand >> 4);
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                mma_ts(tm + 2 * kTile + x * kTile, tm + x * kTile + 8 * c, b0 + c * (2048 >> 4), kIdescMN, it > 0 || c > 0);
+              for (int c = 6; c < 8; ++c) mma_ts(d, p0 + 8 * c, b0 + c * (2048 >> 4), kIdescMN, 1);
               if (x == tiles - 1) tc_commit(&bars->kv_empty[vs]);
               if (it == nt - 1) tc_commit(&bars->o_full[x]);
             }
