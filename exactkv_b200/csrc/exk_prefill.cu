@@ -26,8 +26,13 @@ constexpr int kTile = 128;                 // rows of a query tile, keys of a ke
 constexpr int kHalf = kTile * 128;         // bytes of one operand half: 128 rows x 64 channels bf16
 constexpr int kOperand = 2 * kHalf;        // one operand tile
 constexpr int kSlots = 4;                  // key/value ring: K, V, K, V, ...
-constexpr int kPrefillThreads = 384;       // warps 0-3, 4-7: softmax; 8: MMA; 9: TMA; 10: values of masked tiles; 11: schedule
-constexpr int kRegsSoftmax = 208, kRegsOther = 80;
+// Warps 0-3, 4-7: softmax of the two query tiles; 8-11: output; 12: MMA; 13: TMA;
+// 14: values of masked tiles; 15: schedule. The register split adds up to
+// the launch's 512 threads x 128.
+constexpr int kPrefillThreads = 512;
+constexpr int kMmaWarp = 12, kTmaWarp = 13, kValueWarp = 14;
+constexpr int kReaders = 15;               // warps that read the schedule
+constexpr int kRegsSoftmax = 176, kRegsOutput = 96, kRegsOther = 64;
 constexpr float kRescale = 8.f;            // a row's maximum may grow by 2^8 before O is rescaled
 
 struct PrefillArgs {
@@ -208,7 +213,8 @@ struct Work {
   int tok0, tiles;  // first token of the rows; query tiles in use: 1 or 2
   int keys;         // keys that the last row sees
   int nt, t1;       // key tiles of this split: t1 - 1 down to t1 - nt
-  int masked;       // the first of them, in which some row does not see some key
+  int low;          // keys that every row sees
+  int masked;       // the first of the tiles, in which some row does not see some key
 };
 
 // Item `item` of the grid: (256-row block, KV head, split). Sequence b's blocks take
@@ -252,8 +258,8 @@ __device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int la
   w.t1 = min(all, t0 + per);
   w.nt = w.t1 - t0;
   // tile j holds a key past the first row's last one when (j + 1) * 128 > low
-  const int low = w.L - w.n + w.tok0 + 1;
-  w.masked = min(w.nt, max(0, w.t1 - max(0, low) / kTile));
+  w.low = max(0, w.L - w.n + w.tok0 + 1);
+  w.masked = min(w.nt, max(0, w.t1 - w.low / kTile));
   return true;
 }
 
@@ -276,28 +282,36 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, stop));
 }
 
+// Bits 15 and 31: the half's exponent field is all ones.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+}
+
 struct __align__(16) Bars {
   uint4 answer;
-  uint64_t q_full[2], q_empty[2], kv_full[kSlots], kv_empty[kSlots], v_ok[kSlots], s_full[2], p_most[2], p_full[2], o_full[2];
+  uint64_t q_full[2], q_empty[2], kv_full[kSlots], kv_empty[kSlots], v_ok[kSlots], s_full[2], p_most[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t l_full[2], l_empty[2];
   uint64_t work_full[2], work_empty[2], block, want;
   Work work[2];
+  float l[2][kTile];  // the rows' sums at the end of an item
   uint32_t tmem;
   int stop, bad;
 };
 
-constexpr int kStage = 8 * 32 * 128;
+constexpr int kStage = 4 * 2 * 32 * 128;
 constexpr int kPrefillSmem = 2 * kOperand + kSlots * kOperand + kStage + static_cast<int>(sizeof(Bars)) + 1024;
+static_assert(kPrefillSmem <= 227 * 1024, "one CTA's shared memory");
 
 // The softmax threads' side of one item: query tile x, a row per thread. s_phase:
 // tiles of S this thread has taken so far.
-__device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w, Bars* bars, uint4* stage, uint32_t tmem, int x,
+__device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w, Bars* bars, uint32_t tmem, int x,
                                              uint32_t& s_phase, uint32_t& o_phase, volatile int* stop) {
   const int warp = threadIdx.x >> 5, r = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
   const uint32_t ts = tmem + lanes + x * kTile, to = tmem + lanes + 2 * kTile + x * kTile;
   const int tok = w.tok0 + x * a.tpt + r / a.G;
   const bool valid = r < a.G * a.tpt && tok < w.n;
-  const int lim = valid ? w.L - w.n + tok : -1;  // last key the row sees
+  const int lim = valid ? w.L - w.n + tok : w.keys - 1;  // last key the row sees
   const int nt = w.nt;
   float m = -INFINITY, l = 0.f;
   for (int it = 0; it < nt; ++it) {
@@ -309,10 +323,17 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
     for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
     tc_wait_ld();
     if (it < w.masked) {
+      // columns past the last key the row sees; groups of 32 that every row of the
+      // warp sees are left alone
       const int seen = lim - (w.t1 - 1 - it) * kTile;
+      const int least = __reduce_min_sync(0xFFFFFFFFu, seen);
 #pragma unroll
-      for (int i = 0; i < kTile; ++i)
-        if (i > seen) s[i] = 0xFF800000u;
+      for (int c = 0; c < 4; ++c) {
+        if (least >= 32 * c + 31) continue;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (32 * c + i > seen) s[32 * c + i] = 0xFF800000u;
+      }
     }
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -370,19 +391,46 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
     tc_fence_before();
     mbar_arrive(&bars->p_full[x]);
   }
+  if (nt > 0 && warp_wait(&bars->l_empty[x], (o_phase & 1) ^ 1, stop)) {
+    bars->l[x][r] = l;
+    mbar_arrive(&bars->l_full[x]);
+    if (a.ns > 1 && valid) {
+      const int64_t at = (static_cast<int64_t>(w.first + tok) * a.Hq + w.hk * a.G + r % a.G) * a.ns + w.split;
+      a.pm[at] = m;
+      a.pl[at] = l;
+    }
+  }
+  if (nt > 0) ++o_phase;
+}
+
+// The output warps' side of query tile x: row r = TMEM lane, thread r of the four warps.
+__device__ __forceinline__ void output_item(const PrefillArgs& a, const Work& w, Bars* bars, uint4* stage, uint32_t tmem, int x,
+                                            uint32_t& o_phase, volatile int* stop) {
+  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, r = threadIdx.x & 127;
+  const uint32_t to = tmem + (static_cast<uint32_t>(warp) << 21) + 2 * kTile + x * kTile;
+  const int g = r % a.G, tok = w.tok0 + x * a.tpt + r / a.G;
+  const bool valid = r < a.G * a.tpt && tok < w.n;
+  const int lim = w.L - w.n + tok;
+  const int h = w.hk * a.G + g;
+  const int64_t row = static_cast<int64_t>(w.first + tok) * a.Hq + h;
   bool have = false;
-  if (nt > 0) {
-    have = warp_wait(&bars->o_full[x], o_phase & 1, stop);
-    ++o_phase;
+  float l = 0.f;
+  if (w.nt > 0) {
+    have = warp_wait(&bars->l_full[x], (o_phase >> x) & 1, stop);
+    if (have) {
+      l = bars->l[x][r];
+      mbar_arrive(&bars->l_empty[x]);
+    }
+    have = have && warp_wait(&bars->o_full[x], (o_phase >> x) & 1, stop);
+    o_phase ^= 1u << x;
     tc_fence_after();
   }
-  const int h = w.hk * a.G + r % a.G;
-  const int64_t row = static_cast<int64_t>(w.first + tok) * a.Hq + h;
-  if (a.ns > 1 && valid) {
-    a.pm[row * a.ns + w.split] = have ? m : -INFINITY;
-    a.pl[row * a.ns + w.split] = have ? l : 0.f;
+  if (a.ns > 1 && valid && w.nt == 0) {
+    a.pm[row * a.ns + w.split] = -INFINITY;
+    a.pl[row * a.ns + w.split] = 0.f;
   }
-  const float inv = a.ns > 1 ? 1.f : (have && l > 0.f ? 1.f / l : (l != l ? l : 0.f));
+  // (a NaN sum makes the row NaN; a row without keys becomes 0)
+  const float inv = a.ns > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
   const bool bad = *const_cast<volatile int*>(&bars->bad) != 0;
   // The row's place; null: not written (no row, or a split without keys).
   uint64_t dst = 0;
@@ -392,18 +440,15 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
   // 128 bytes of every row at a time go through shared memory, 16-byte pieces
   // swizzled by row, so that eight lanes write a whole line: stored by the rows'
   // own threads, 16 bytes a row, the tile took 6,000 cycles.
-  uint4* mine = stage + warp * 256;
-  const int lane = threadIdx.x & 31;
+  uint4* mine = stage + warp * 512;
   auto flush = [&](int part) {
-    __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int from = 4 * i + (lane >> 3);
       const uint64_t d = __shfl_sync(0xFFFFFFFFu, dst, from);
-      const uint4 v = mine[from * 8 + ((lane & 7) ^ (from & 7))];
+      const uint4 v = mine[(part & 1) * 256 + from * 8 + ((lane & 7) ^ (from & 7))];
       if (d != 0) reinterpret_cast<uint4*>(d + 128 * part)[lane & 7] = v;
     }
-    __syncwarp();
   };
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
@@ -414,11 +459,11 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
     }
     float f[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = have && !(l == 0.f) ? __uint_as_float(o[i]) * inv : 0.f;
+    for (int i = 0; i < 32; ++i) f[i] = l == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
     if (bad && valid) {
       // a masked tile held values that are not finite: they were left out of
       // the product and reach the rows that see them here
-      for (int t = (w.t1 - w.masked) * kTile; t < min(w.t1 * kTile, lim + 1); ++t) {
+      for (int t = max(w.low, (w.t1 - w.nt) * kTile); t < min(w.t1 * kTile, lim + 1); ++t) {
         int64_t vrow = static_cast<int64_t>(w.krow) + t;
         if (a.block_table != nullptr) {
           const int pg = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + t / kP);
@@ -434,19 +479,29 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
     if (a.ns > 1) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        mine[lane * 8 + (i ^ (lane & 7))] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]),
-                                                       __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+        mine[(c & 1) * 256 + lane * 8 + (i ^ (lane & 7))] =
+            make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
+                       __float_as_uint(f[4 * i + 3]));
+      __syncwarp();
       flush(c);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        mine[lane * 8 + ((4 * (c & 1) + i) ^ (lane & 7))] =
+        mine[(c >> 1) * 256 + lane * 8 + ((4 * (c & 1) + i) ^ (lane & 7))] =
             make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
                        pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
-      if (c & 1) flush(c >> 1);
     }
   }
-  tc_fence_before();
+  if (have) {  // the next item may write O
+    tc_fence_before();
+    mbar_arrive(&bars->o_empty[x]);
+  }
+  if (a.ns == 1) {
+    __syncwarp();
+    flush(0);
+    flush(1);
+  }
+  __syncwarp();
 }
 
 // One CTA per SM, which takes blocks of the grid as they come (longest first):
@@ -458,7 +513,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   uint8_t* sq = smem;
   uint8_t* ring = smem + 2 * kOperand;
-  uint4* stage = reinterpret_cast<uint4*>(ring + kSlots * kOperand);  // 32 rows of 128 bytes for each softmax warp
+  uint4* stage = reinterpret_cast<uint4*>(ring + kSlots * kOperand);  // 2 x 32 rows of 128 bytes for each output warp
   Bars* bars = reinterpret_cast<Bars*>(ring + kSlots * kOperand + kStage);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* stop = &bars->stop;
@@ -472,11 +527,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       mbar_init(&bars->p_full[i], kTile);
       mbar_init(&bars->o_full[i], 1);
       mbar_init(&bars->work_full[i], 1);
-      mbar_init(&bars->work_empty[i], 11);
+      mbar_init(&bars->work_empty[i], kReaders);
+      mbar_init(&bars->o_empty[i], kTile);
+      mbar_init(&bars->l_full[i], kTile);
+      mbar_init(&bars->l_empty[i], kTile);
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&bars->kv_full[i], 1);
-      mbar_init(&bars->kv_empty[i], 1 + (i & 1));  // V entries (odd): the products and warp 10
+      mbar_init(&bars->kv_empty[i], 1 + (i & 1));  // V entries (odd): the products and the value warp
       mbar_init(&bars->v_ok[i], 32);
     }
     mbar_init(&bars->block, 1);
@@ -484,7 +542,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     bars->stop = bars->bad = 0;
     fence_mbar_init();
   }
-  if (warp == 8) tmem_alloc(&bars->tmem, 512);
+  if (warp == kMmaWarp) tmem_alloc(&bars->tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -507,14 +565,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     uint32_t s_phase = 0, o_phase = 0;
     Work w;
     while (next_work(w))
-      if (x < w.tiles) softmax_item(a, w, bars, stage, tmem, x, s_phase, o_phase, stop);
+      if (x < w.tiles) softmax_item(a, w, bars, tmem, x, s_phase, o_phase, stop);
+  } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOutput));
+    uint32_t o_phase = 0;
+    Work w;
+    while (next_work(w))
+      for (int x = 0; x < w.tiles; ++x) output_item(a, w, bars, stage, tmem, x, o_phase, stop);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
       // ---- MMA: K of an item's tile `it` is ring entry e + 2 it, V the one after
       const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
       const uint64_t dq = desc_kmajor(smem_addr(sq)), dk = desc_kmajor(smem_addr(ring)), dv = desc_mnmajor(smem_addr(ring));
-      uint32_t e = 0, q_phase = 0, p_phase = 0, ok_phase = 0;  // bit x (or slot): the parity to wait for next
+      uint32_t e = 0, q_phase = 0, p_phase = 0, o_phase = 3, ok_phase = 0;  // bit x (or slot): the parity to wait for next
       // S of query tile x from the K in `slot`; `last`: the item's last use of Q
       auto qk = [&](int x, uint32_t slot, bool last) {
         if (elect_one()) {
@@ -555,7 +619,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             // beside the last exponentials
             const uint64_t b0 = dv + vs * (kOperand >> 4);
             const uint32_t d = tm + 2 * kTile + x * kTile, p0 = tm + x * kTile;
-            ok = warp_wait(&bars->p_most[x], (p_phase >> x) & 1, stop);
+            if (it == 0) {  // the item before has been read out of O
+              ok = warp_wait(&bars->o_empty[x], (o_phase >> x) & 1, stop);
+              o_phase ^= 1u << x;
+            }
+            ok = ok && warp_wait(&bars->p_most[x], (p_phase >> x) & 1, stop);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
@@ -584,7 +652,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         e += 2 * nt;
         if (!ok) break;
       }
-    } else if (warp == 9) {
+    } else if (warp == kTmaWarp) {
       // ---- TMA
       const int tile_bytes = 64 * 2 * a.G * a.tpt;
       uint32_t e = 0, q_phase = 3;
@@ -644,9 +712,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (!ok) break;
         if (lane == 0) mbar_arrive(&bars->want);
       }
-    } else if (warp == 10) {
+    } else if (warp == kValueWarp) {
       // ---- values of masked tiles: rows past the last key become zeros, and so do
-      // values that are not finite (0 x inf would reach rows that do not see them)
+      // values that are not finite and that some row does not see (0 x inf is NaN). Only
+      // such rows are looked at, up to 64 of 128 with four heads to a group: a look
+      // at every piece by itself held the products up for 8,000 cycles an item.
       uint32_t e = 0;
       Work w;
       while (next_work(w)) {
@@ -661,28 +731,32 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             if (lane == 0) mbar_arrive(&bars->kv_empty[vs]);
             continue;
           }
+          // the tile's rows [open, end): keys that some of the item's rows see and some do not
+          const int base = (w.t1 - 1 - it) * kTile;
+          const int open = max(0, w.low - base), end = min(kTile, w.keys - base);
           uint4* v = reinterpret_cast<uint4*>(ring + vs * kOperand);
           bool bad = false;
-          const int rows = w.keys - (w.t1 - 1 - it) * kTile;  // keys of the tile that some row sees
-#pragma unroll 4
-          for (int i = lane; i < kOperand / 16; i += 32) {
-            const int row = (i >> 3) & (kTile - 1);
-            if (row >= rows) {
-              v[i] = make_uint4(0, 0, 0, 0);
-            } else {
-              // bit 15 of each half: exponent field all ones
-              uint4 u = v[i];
-              const uint32_t b0 = ((u.x & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-              const uint32_t b1 = ((u.y & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-              const uint32_t b2 = ((u.z & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-              const uint32_t b3 = ((u.w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-              if ((b0 | b1 | b2 | b3) != 0u) {
-                u.x &= ~((b0 >> 15) * 0xFFFFu);
-                u.y &= ~((b1 >> 15) * 0xFFFFu);
-                u.z &= ~((b2 >> 15) * 0xFFFFu);
-                u.w &= ~((b3 >> 15) * 0xFFFFu);
-                v[i] = u;
-                bad = true;
+          for (int half = 0; half < 2; ++half, v += kHalf / 16) {
+            for (int i = 8 * end + lane; i < 8 * kTile; i += 32) v[i] = make_uint4(0, 0, 0, 0);
+            // eight pieces in flight at once; what is found is cleared in a second look
+            for (int i0 = 8 * open + lane; i0 < 8 * end; i0 += 256) {
+              uint4 u[8];
+#pragma unroll
+              for (int c = 0; c < 8; ++c) u[c] = i0 + 32 * c < 8 * end ? v[i0 + 32 * c] : make_uint4(0, 0, 0, 0);
+              uint32_t any = 0u;
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                any |= not_finite(u[c].x) | not_finite(u[c].y) | not_finite(u[c].z) | not_finite(u[c].w);
+              if (any == 0u) continue;
+              bad = true;
+#pragma unroll 1
+              for (int i = i0; i < min(8 * end, i0 + 256); i += 32) {
+                uint4 x = v[i];
+                x.x &= ~((not_finite(x.x) >> 15) * 0xFFFFu);
+                x.y &= ~((not_finite(x.y) >> 15) * 0xFFFFu);
+                x.z &= ~((not_finite(x.z) >> 15) * 0xFFFFu);
+                x.w &= ~((not_finite(x.w) >> 15) * 0xFFFFu);
+                v[i] = x;
               }
             }
           }
@@ -738,7 +812,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     if (threadIdx.x == 0) set_status(a.status, EXK_S_FULL_TIMEOUT);
     __syncthreads();
   }
-  if (warp == 8) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_free(tmem, 512);
   }
