@@ -6,6 +6,7 @@ nonzero return code into RuntimeError.
 """
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libexactkv_b200.so")
@@ -29,19 +30,11 @@ class Partials(ctypes.Structure):
                 ("heads", c_int32)]
 
 
-class Append(ctypes.Structure):
-    """exk_append: the packed new tokens of a batch and where they go."""
-    _fields_ = [(n, c_void_p) for n in ("q", "k", "v", "q_out")] + \
-               [(n, c_int64) for n in ("q_st", "q_sh", "k_st", "k_sh", "v_st", "v_sh", "o_st", "o_sh")] + \
-               [(n, c_void_p) for n in ("cos_sin", "q_norm", "k_norm", "cu_seqlens", "seq_lens", "block_table", "slots")] + \
-               [(n, c_int32) for n in ("N", "B", "Hq", "Hkv", "rope_rows", "max_pages", "pool_pages")] + [("eps", c_float)]
-
-
-class Prefill(ctypes.Structure):
-    """exk_prefill: packed queries, output and split partials of a prompt attention."""
-    _fields_ = [("q", c_void_p), ("out", c_void_p)] + [(n, c_int64) for n in ("q_st", "q_sh", "o_st", "o_sh")] + \
-               [(n, c_void_p) for n in ("cu_q", "po", "pm", "pl")] + \
-               [(n, c_int32) for n in ("N", "B", "Hq", "Hkv", "ns")] + [("qk_scale", c_float)]
+# exk_append and exk_prefill as packed bytes (building a ctypes.Structure of 31
+# fields takes several times as long as the call that reads it).
+APPEND = struct.Struct("@4P8q7P7if")     # q k v q_out; 8 strides; cos_sin .. slots; N .. pool_pages; eps
+CVIEW = struct.Struct("@6Pq")            # exk_cview
+PREFILL = struct.Struct("@2P4q4P5if")    # q out; 4 strides; cu_q po pm pl; N B Hq Hkv ns; qk_scale
 
 
 _P = ctypes.POINTER
@@ -87,16 +80,16 @@ _SIGNATURES.update({
     "exk_selftest_wait_timeout": (c_int, [c_void_p, ctypes.c_uint64, c_int, c_void_p]),
     "exk_attention_compressed_noalloc": (c_int, [c_void_p, _P(CView), _P(CView), c_int, c_int, c_int, c_int, c_int,
                                                  c_int, c_float, c_void_p, c_void_p, c_int, c_void_p]),
-    "exk_rope_append_bf16": (c_int, [_P(Append), c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "exk_rope_append_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "exk_rope_append_scratch": (c_int64, [c_int, c_int, c_int, c_int]),
-    "exk_rope_append_compressed": (c_int, [_P(Append), _P(CView), c_int64, c_void_p, _P(CView), c_int64, c_void_p,
+    "exk_rope_append_compressed": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
                                            c_void_p, c_int64, c_void_p, c_int, c_void_p]),
     "exk_prefill_splits": (c_int, [c_int, c_int, c_int, c_int, c_int64, c_int]),
-    "exk_attention_prefill": (c_int, [_P(Prefill), c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int,
+    "exk_attention_prefill": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int,
                                       c_void_p, c_void_p, c_int, c_void_p]),
-    "exk_attention_prefill_paged": (c_int, [_P(Prefill), c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
+    "exk_attention_prefill_paged": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                             c_void_p, c_int, c_void_p]),
-    "exk_attention_prefill_paged_compressed": (c_int, [_P(Prefill), _P(CView), _P(CView), c_int, c_void_p, c_int,
+    "exk_attention_prefill_paged_compressed": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                                        c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                                        c_void_p]),
     "exk_error_string": (ctypes.c_char_p, [c_int]),

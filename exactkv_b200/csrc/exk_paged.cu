@@ -30,7 +30,8 @@ struct Append {
   int64_t cap[2];
   int32_t* cnt[2];
   int32_t tails;      // open pages per KV head that the raw pools hold
-  uint8_t* counts;    // [2][items_pad] raw rows of every item (scratch)
+  uint8_t* counts;    // [2][items_pad] raw rows of every item, and its flags (scratch)
+  int2* pages;        // [items] where the item completed its page: its entry of the page arrays, its sequence (scratch)
   int32_t* base_cnt;  // [2] the pools' counters before this call (scratch)
   int32_t slots;      // page slots of the call (see page_slot)
   int32_t items;      // slots * Hkv
@@ -83,153 +84,188 @@ __device__ __forceinline__ int pool_page(const Append& a, int b, int pg) {
 
 // ---------------------------------------------------------------- rotation
 
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+// -0 that the compiler does not know: x y + (-0) is the rounded product, kept
+// from being fused with the sum that follows (a packed product and a packed sum,
+// both .rn, come out as one packed fma).
+static __constant__ float c_minus_zero = -0.f;
 
-// The pair (x_j, x_{j+64}) rotated.
-__device__ __forceinline__ void rotate(float& lo, float& hi, float c, float s) {
-  const float l = lo, h = hi;
-  lo = __fsub_rn(__fmul_rn(l, c), __fmul_rn(h, s));
-  hi = __fadd_rn(__fmul_rn(h, c), __fmul_rn(l, s));
+// Cosines and sines of 2 NW consecutive channels, as pairs; sines negated too:
+// l c - h s is formed as l c + h (-s), the same bits, so that two channels at a
+// time are rotated by packed products and sums.
+template <int NW>
+struct Turn {
+  F2 c[NW], s[NW], ns[NW];
+};
+
+__device__ __forceinline__ float4 ldg4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
+
+// Channels c0 .. c0 + 2 NW - 1 of the table's row `cs`.
+template <int NW>
+__device__ __forceinline__ void load_turn(const float* cs, int c0, Turn<NW>& t) {
+#pragma unroll
+  for (int j = 0; j < NW; j += 2) {
+    const float4 c = ldg4(cs + c0 + 2 * j), s = ldg4(cs + 64 + c0 + 2 * j);
+    t.c[j] = f2(c.x, c.y);
+    t.c[j + 1] = f2(c.z, c.w);
+    t.s[j] = f2(s.x, s.y);
+    t.s[j + 1] = f2(s.z, s.w);
+    t.ns[j] = f2(-s.x, -s.y);
+    t.ns[j + 1] = f2(-s.z, -s.w);
+  }
 }
 
-// NW packed words of each half (channels c0 .. c0 + 2 NW - 1 and those + 64)
-// of one head, held by LANES lanes of a group: normalised (w != nullptr) and
-// rotated. cs: the position's row of the table.
-template <int NW, int LANES>
-__device__ __forceinline__ void norm_rotate(uint32_t (&lo)[NW], uint32_t (&hi)[NW], int c0, const uint16_t* w, float eps,
-                                            const float (&c)[2 * NW], const float (&s)[2 * NW]) {
-  float x[2 * NW], y[2 * NW];
+// One head held by a group of lanes, NW packed words of each half (channels c0 ..
+// c0 + 2 NW - 1 and those + 64) to a lane: this lane's part of its sum of squares.
+template <int NW>
+__device__ __forceinline__ float squares(const uint32_t (&lo)[NW], const uint32_t (&hi)[NW]) {
+  F2 ss = f2(0.f, 0.f);
 #pragma unroll
   for (int j = 0; j < NW; ++j) {
-    x[2 * j] = bf_lo(lo[j]);
-    x[2 * j + 1] = bf_hi(lo[j]);
-    y[2 * j] = bf_lo(hi[j]);
-    y[2 * j + 1] = bf_hi(hi[j]);
+    const F2 x = f2_bf16(lo[j]), y = f2_bf16(hi[j]);
+    ss = fma2(y, y, fma2(x, x, ss));
   }
-  if (w != nullptr) {
-    float ss = 0.f;
+  float s0, s1;
+  split2(ss, s0, s1);
+  return s0 + s1;
+}
+
+// The head rotated, after the norm by weight w where NORM: r = 1 / sqrt(mean square + eps).
+template <int NW, bool NORM>
+__device__ __forceinline__ void norm_rotate(uint32_t (&lo)[NW], uint32_t (&hi)[NW], int c0, const uint16_t* w, float r,
+                                            const Turn<NW>& t) {
+  F2 x[NW], y[NW];
 #pragma unroll
-    for (int j = 0; j < 2 * NW; ++j) ss += x[j] * x[j] + y[j] * y[j];
+  for (int j = 0; j < NW; ++j) {
+    x[j] = f2_bf16(lo[j]);
+    y[j] = f2_bf16(hi[j]);
+  }
+  if constexpr (NORM) {
+    const F2 rr = f2(r, r);
 #pragma unroll
-    for (int d = LANES / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
-    const float r = rsqrtf(ss * (1.f / kD) + eps);
-#pragma unroll
-    for (int j = 0; j < 2 * NW; ++j) {
-      x[j] = x[j] * r * __uint_as_float(static_cast<uint32_t>(__ldg(w + c0 + j)) << 16);
-      y[j] = y[j] * r * __uint_as_float(static_cast<uint32_t>(__ldg(w + 64 + c0 + j)) << 16);
+    for (int j = 0; j < NW; j += 2) {
+      const uint2 a = __ldg(reinterpret_cast<const uint2*>(w + c0 + 2 * j));
+      const uint2 b = __ldg(reinterpret_cast<const uint2*>(w + 64 + c0 + 2 * j));
+      x[j] = mul2(mul2(x[j], rr), f2_bf16(a.x));
+      x[j + 1] = mul2(mul2(x[j + 1], rr), f2_bf16(a.y));
+      y[j] = mul2(mul2(y[j], rr), f2_bf16(b.x));
+      y[j + 1] = mul2(mul2(y[j + 1], rr), f2_bf16(b.y));
     }
   }
-#pragma unroll
-  for (int j = 0; j < 2 * NW; ++j) rotate(x[j], y[j], c[j], s[j]);
+  const float mz = c_minus_zero;
+  const F2 z = f2(mz, mz);
 #pragma unroll
   for (int j = 0; j < NW; ++j) {
-    lo[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
-    hi[j] = pack_bf16x2(y[2 * j], y[2 * j + 1]);
+    lo[j] = bf16_f2(add2(fma2(x[j], t.c[j], z), fma2(y[j], t.ns[j], z)));
+    hi[j] = bf16_f2(add2(fma2(y[j], t.c[j], z), fma2(x[j], t.s[j], z)));
   }
-}
-
-__device__ __forceinline__ void load4(float* d, const float* s) {
-  const float4 v = __ldg(reinterpret_cast<const float4*>(s));
-  d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
 }
 
 // ---------------------------------------------------------------- rows of a token
 
-constexpr int kRowWarps = 8;
-constexpr int kQuads = 2;  // groups of four heads one warp takes
+constexpr int kRowWarps = 4;
+// Groups of four heads that a warp has in flight at once: four with 124 registers
+// (11,016 tokens of 48 heads: 44.3 us, 6.2 TB/s; two: 49.0 us); the norm's
+// shuffles make two with more warps better (50.3 us; four: 61.4 us).
+template <bool NORM>
+constexpr int kQuads = NORM ? 2 : 4;
 
-// One warp: heads 4 * quad0 .. of one token (the queries' heads, then, with
-// KV, the keys' and the values'), eight lanes to a head, 16 bytes of each half
-// to a lane.
-template <bool KV>
-__device__ __forceinline__ void token_rows(const Append& a, int64_t work, int lane) {
+// One warp: `steps` times 4 * kQuads heads of one token (the queries' heads,
+// then, with KV, the keys' and the values'), eight lanes to a head, 16 bytes of
+// each half to a lane. The first heads are loaded before the token's sequence
+// is looked up, and every step's while the step before is rotated.
+template <bool KV, bool NORM>
+__device__ __forceinline__ void token_rows(const Append& a, int64_t work, int steps, int lane) {
+  constexpr int Q = kQuads<NORM>;
   const exk_append& t = a.t;
   const int heads = t.Hq + (KV ? 2 * t.Hkv : 0);
-  const int per_token = (heads + 4 * kQuads - 1) / (4 * kQuads);
+  const int per_token = (heads + 4 * Q * steps - 1) / (4 * Q * steps);
   const int tok = static_cast<int>(work / per_token);
   if (tok >= t.N) return;
-  const int h0 = static_cast<int>(work % per_token) * (4 * kQuads) + (lane >> 3);
+  int base = static_cast<int>(work % per_token) * (4 * Q * steps);
+  const int sub = lane >> 3, c0 = 8 * (lane & 7);
+  uint4 lo[Q], hi[Q];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+      const int h = from + 4 * u + sub;
+      const uint16_t* src = nullptr;
+      if (h < t.Hq)
+        src = t.q + tok * t.q_st + h * t.q_sh;
+      else if (KV && h < t.Hq + t.Hkv)
+        src = t.k + tok * t.k_st + (h - t.Hq) * t.k_sh;
+      else if (KV && h < heads)
+        src = t.v + tok * t.v_st + (h - t.Hq - t.Hkv) * t.v_sh;
+      lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
+      if (src != nullptr) {
+        lo[u] = *reinterpret_cast<const uint4*>(src + c0);
+        hi[u] = *reinterpret_cast<const uint4*>(src + 64 + c0);
+      }
+    }
+  };
+  load(base);
   const int b = t.cu_seqlens == nullptr ? tok : find_seq(t.cu_seqlens, t.B, 1, 0, tok, lane);
   if (b >= t.B) return;  // behind the last sequence
   const Seq s = load_seq(t, b);
   if (s.n <= 0) return;
   const int pos = s.start + tok - s.first;
   const bool ok = position_ok(t, pos);
-  const int c0 = 8 * (lane & 7);
-  float c[8], sn[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) c[j] = sn[j] = 0.f;
+  Turn<4> turn;
   int64_t row = -1;
-  if (ok) {
-    const float* cs = t.cos_sin + static_cast<int64_t>(pos) * kD + c0;
-    load4(c, cs);
-    load4(c + 4, cs + 4);
-    load4(sn, cs + 64);
-    load4(sn + 4, cs + 68);
-    if (KV) {
-      const int page = pool_page(a, b, pos / kP);
-      if (page >= 0) row = static_cast<int64_t>(page) * kP + pos % kP;
-    }
-  } else {
+  load_turn(t.cos_sin + static_cast<int64_t>(ok ? pos : 0) * kD, c0, turn);
+  if (!ok) {
     set_status(a.status, EXK_S_POSITION);
+  } else if (KV) {
+    const int page = pool_page(a, b, pos / kP);
+    if (page >= 0) row = static_cast<int64_t>(page) * kP + pos % kP;
   }
-  uint32_t lo[kQuads][4], hi[kQuads][4];
+  for (; steps > 0 && base < heads; --steps, base += 4 * Q) {
+    uint32_t l[Q][4], g[Q][4];
+    float r[Q];
 #pragma unroll
-  for (int u = 0; u < kQuads; ++u) {
-    const int h = h0 + 4 * u;
-    const uint16_t* src = nullptr;
-    if (h < t.Hq)
-      src = t.q + tok * t.q_st + h * t.q_sh;
-    else if (KV && h < t.Hq + t.Hkv)
-      src = t.k + tok * t.k_st + (h - t.Hq) * t.k_sh;
-    else if (KV && h < heads)
-      src = t.v + tok * t.v_st + (h - t.Hq - t.Hkv) * t.v_sh;
-    uint4 l = make_uint4(0, 0, 0, 0), g = l;
-    if (src != nullptr) {
-      l = *reinterpret_cast<const uint4*>(src + c0);
-      g = *reinterpret_cast<const uint4*>(src + 64 + c0);
+    for (int u = 0; u < Q; ++u) {
+      l[u][0] = lo[u].x; l[u][1] = lo[u].y; l[u][2] = lo[u].z; l[u][3] = lo[u].w;
+      g[u][0] = hi[u].x; g[u][1] = hi[u].y; g[u][2] = hi[u].z; g[u][3] = hi[u].w;
+      r[u] = 0.f;
     }
-    lo[u][0] = l.x; lo[u][1] = l.y; lo[u][2] = l.z; lo[u][3] = l.w;
-    hi[u][0] = g.x; hi[u][1] = g.y; hi[u][2] = g.z; hi[u][3] = g.w;
-  }
+    if (steps > 1) load(base + 4 * Q);
+    if constexpr (NORM) {  // every quad's sums together: their shuffles do not wait on one another
 #pragma unroll
-  for (int u = 0; u < kQuads; ++u) {
-    const int h = h0 + 4 * u;
-    if (h - (lane >> 3) >= heads) break;  // whole warp
-    // a warp's four heads may be of two kinds: every lane runs the same
-    // shuffles, and a value head keeps what it loaded
-    const bool value = KV && h >= t.Hq + t.Hkv;
-    uint32_t rl[4], rh[4];
+      for (int u = 0; u < Q; ++u) r[u] = squares<4>(l[u], g[u]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      rl[j] = lo[u][j];
-      rh[j] = hi[u][j];
+      for (int d = 4; d > 0; d >>= 1) {
+#pragma unroll
+        for (int u = 0; u < Q; ++u) r[u] += __shfl_xor_sync(0xFFFFFFFFu, r[u], d);
+      }
+#pragma unroll
+      for (int u = 0; u < Q; ++u) r[u] = rsqrtf(r[u] * (1.f / kD) + t.eps);
     }
-    if (t.q_norm != nullptr || t.k_norm != nullptr) {
-      // both norms or none (checked on the host)
-      norm_rotate<4, 8>(rl, rh, c0, h < t.Hq ? t.q_norm : t.k_norm, t.eps, c, sn);
-    } else {
-      norm_rotate<4, 8>(rl, rh, c0, nullptr, 0.f, c, sn);
-    }
-    uint16_t* dst = nullptr;
-    if (h < t.Hq)
-      dst = t.q_out + tok * t.o_st + h * t.o_sh;
-    else if (KV && row >= 0 && h < heads)
-      dst = a.pool[value ? 1 : 0] + (row * t.Hkv + (h - t.Hq - (value ? t.Hkv : 0))) * kD;
-    if (dst == nullptr) continue;
-    if (value) {
-      *reinterpret_cast<uint4*>(dst + c0) = make_uint4(lo[u][0], lo[u][1], lo[u][2], lo[u][3]);
-      *reinterpret_cast<uint4*>(dst + 64 + c0) = make_uint4(hi[u][0], hi[u][1], hi[u][2], hi[u][3]);
-    } else {
-      *reinterpret_cast<uint4*>(dst + c0) = make_uint4(rl[0], rl[1], rl[2], rl[3]);
-      *reinterpret_cast<uint4*>(dst + 64 + c0) = make_uint4(rh[0], rh[1], rh[2], rh[3]);
+#pragma unroll
+    for (int u = 0; u < Q; ++u) {
+      const int h = base + 4 * u + sub;
+      uint16_t* dst = nullptr;
+      if (h < t.Hq + (KV ? t.Hkv : 0)) {
+        norm_rotate<4, NORM>(l[u], g[u], c0, h < t.Hq ? t.q_norm : t.k_norm, r[u], turn);
+        if (h < t.Hq)
+          dst = t.q_out + tok * t.o_st + h * t.o_sh;
+        else if (row >= 0)
+          dst = a.pool[0] + (row * t.Hkv + (h - t.Hq)) * kD;
+        if (!ok) {  // (queries alone get here)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) l[u][j] = g[u][j] = 0u;
+        }
+      } else if (KV && h < heads && row >= 0) {
+        dst = a.pool[1] + (row * t.Hkv + (h - t.Hq - t.Hkv)) * kD;
+      }
+      if (dst == nullptr) continue;
+      *reinterpret_cast<uint4*>(dst + c0) = make_uint4(l[u][0], l[u][1], l[u][2], l[u][3]);
+      *reinterpret_cast<uint4*>(dst + 64 + c0) = make_uint4(g[u][0], g[u][1], g[u][2], g[u][3]);
     }
   }
 }
 
-__global__ void __launch_bounds__(kRowWarps * 32) append_bf16_kernel(const __grid_constant__ Append a) {
-  token_rows<true>(a, static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5), threadIdx.x & 31);
+template <bool NORM>
+__global__ void __launch_bounds__(kRowWarps * 32) append_bf16_kernel(const __grid_constant__ Append a, int steps) {
+  token_rows<true, NORM>(a, static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5), steps, threadIdx.x & 31);
 }
 
 // ---------------------------------------------------------------- coded pools
@@ -246,6 +282,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) append_bf16_kernel(const __gri
 // escaped rows. A call that completes a page whose earlier rows are in the
 // tail and leaves another page open writes the latter's rows in the second
 // kernel, by the warp that has copied the former's escaped rows.
+
+// In an item's count byte: the call completed the page; the item's warp in the
+// second kernel also writes the sequence's open page.
+constexpr int kItemFull = 0x20, kItemOpens = 0x40, kItemRows = 0x1F;
 
 struct Item {
   Seq s;
@@ -288,26 +328,49 @@ __device__ __forceinline__ Item load_item(const Append& a, int item, int lane) {
   return it;
 }
 
-// The lane's channels (4q.. and 64 + 4q..) of packed token tok, KV head h, as
-// the cache holds them: keys (which = 0) normalised and rotated at pos.
-__device__ __forceinline__ void cache_row(const Append& a, int which, int tok, int h, int pos, int q, uint32_t (&w)[4]) {
+// `it` completes its sequence's first page, whose earlier rows are in the tail,
+// and the sequence's last page stays open: that one is written after `it`.
+__device__ __forceinline__ bool opens_later(const Item& it) {
+  const int last = last_page(it.s);
+  return it.pg == it.s.start / kP && it.s.start % kP != 0 && last > it.pg && (last + 1) * kP > it.s.start + it.s.n;
+}
+
+// The lane's channels (4q.. and 64 + 4q..) of packed token tok, KV head h: keys
+// (which = 0) or values.
+__device__ __forceinline__ void load_quads(const Append& a, int which, int tok, int h, int q, uint32_t (&w)[4]) {
   const exk_append& t = a.t;
   const uint16_t* src = which == 0 ? t.k + tok * t.k_st + h * t.k_sh : t.v + tok * t.v_st + h * t.v_sh;
   const uint2 lo = *reinterpret_cast<const uint2*>(src + 4 * q);
   const uint2 hi = *reinterpret_cast<const uint2*>(src + 64 + 4 * q);
-  uint32_t l[2] = {lo.x, lo.y}, g[2] = {hi.x, hi.y};
-  if (which == 0) {
-    float c[4], s[4];
-    const float* cs = t.cos_sin + static_cast<int64_t>(pos) * kD + 4 * q;
-    load4(c, cs);
-    load4(s, cs + 64);
-    norm_rotate<2, 16>(l, g, 4 * q, t.k_norm, t.eps, c, s);
+  w[0] = lo.x; w[1] = lo.y; w[2] = hi.x; w[3] = hi.y;
+}
+
+// They as the cache holds them: keys normalised and rotated at pos (whole warp).
+template <bool NORM>
+__device__ __forceinline__ void cache_form(const Append& a, int which, int pos, int q, uint32_t (&w)[4]) {
+  if (which != 0) return;
+  uint32_t l[2] = {w[0], w[1]}, g[2] = {w[2], w[3]};
+  Turn<2> turn;
+  load_turn(a.t.cos_sin + static_cast<int64_t>(pos) * kD, 4 * q, turn);
+  float r = 0.f;
+  if constexpr (NORM) {
+    r = squares<2>(l, g);
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) r += __shfl_xor_sync(0xFFFFFFFFu, r, d);
+    r = rsqrtf(r * (1.f / kD) + a.t.eps);
   }
+  norm_rotate<2, NORM>(l, g, 4 * q, a.t.k_norm, r, turn);
   w[0] = l[0]; w[1] = l[1]; w[2] = g[0]; w[3] = g[1];
 }
 
 __device__ __forceinline__ uint16_t* tail_row(const Append& a, int which, int slot, int h, int r) {
   return a.raw[which] + (a.cap[which] + (static_cast<int64_t>(slot) * a.t.Hkv + h) * kP + r) * kD;
+}
+
+__device__ __forceinline__ void load_tail(const Append& a, int which, int slot, int h, int r, int q, uint32_t (&w)[4]) {
+  const uint16_t* s = tail_row(a, which, slot, h, r);
+  const uint2 lo = *reinterpret_cast<const uint2*>(s + 4 * q), hi = *reinterpret_cast<const uint2*>(s + 64 + 4 * q);
+  w[0] = lo.x; w[1] = lo.y; w[2] = hi.x; w[3] = hi.y;
 }
 
 __device__ __forceinline__ void store_quads(uint16_t* d, int q, const uint32_t (&w)[4]) {
@@ -317,17 +380,24 @@ __device__ __forceinline__ void store_quads(uint16_t* d, int q, const uint32_t (
 
 // The new rows of an open page into the sequence's tail rows, and the page's
 // entry: all rows raw, at the tail rows.
+template <bool NORM>
 __device__ __forceinline__ void write_open(const Append& a, const Item& it, int which, int lane) {
   const int q = lane & 15, th = lane >> 4;
-  const int end = it.s.start + it.s.n;
-  // two rows at a time, one per half warp; the norm's shuffles need every lane
-  for (int r = max(0, it.s.start - it.pg * kP) & ~1; it.pg * kP + r < end; r += 2) {
-    const int pos = it.pg * kP + r + th;
-    const bool mine = pos >= it.s.start && pos < end;
-    const int at = min(max(pos, it.s.start), end - 1);
-    uint32_t w[4];
-    cache_row(a, which, it.s.first + at - it.s.start, it.h, at, q, w);
-    if (mine) store_quads(tail_row(a, which, it.slot, it.h, r + th), q, w);
+  const int first = it.s.start - it.pg * kP, end = it.s.start + it.s.n - it.pg * kP;  // new rows of the page
+  uint32_t w[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 8 * th + i;
+    w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0u;
+    if (r >= first && r < end) load_quads(a, which, it.s.first + r - first, it.h, q, w[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 8 * th + i;
+    const bool mine = r >= first && r < end;
+    if (!__any_sync(0xFFFFFFFFu, mine)) continue;
+    cache_form<NORM>(a, which, it.pg * kP + min(r, end - 1), q, w[i]);
+    if (mine) store_quads(tail_row(a, which, it.slot, it.h, r), q, w[i]);
   }
   if (lane == 0) {
     const int64_t page = static_cast<int64_t>(it.pool) * a.t.Hkv + it.h;
@@ -337,11 +407,12 @@ __device__ __forceinline__ void write_open(const Append& a, const Item& it, int 
 }
 
 // Blocks below `enc_blocks`: the items; the others rotate the queries.
-__global__ void __launch_bounds__(kRowWarps * 32) append_encode_kernel(const __grid_constant__ Append a, int enc_blocks) {
+template <bool NORM>
+__global__ void __launch_bounds__(kRowWarps * 32) append_encode_kernel(const __grid_constant__ Append a, int enc_blocks, int steps) {
   allow_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (static_cast<int>(blockIdx.x) >= enc_blocks) {
-    token_rows<false>(a, static_cast<int64_t>(blockIdx.x - enc_blocks) * kRowWarps + warp, lane);
+    token_rows<false, NORM>(a, static_cast<int64_t>(blockIdx.x - enc_blocks) * kRowWarps + warp, steps, lane);
     return;
   }
   if (blockIdx.x == 0 && threadIdx.x < 2) a.base_cnt[threadIdx.x] = *a.cnt[threadIdx.x];
@@ -354,15 +425,21 @@ __global__ void __launch_bounds__(kRowWarps * 32) append_encode_kernel(const __g
     const int q = lane & 15, th = lane >> 4;
     uint32_t w[8][4];
 #pragma unroll
+    for (int i = 0; i < 8; ++i) {  // (rows of the page that this call does not bring come from the tail, as they are)
+      const int pos = it.pg * kP + 8 * th + i;
+      if (pos >= it.s.start)
+        load_quads(a, which, it.s.first + pos - it.s.start, it.h, q, w[i]);
+      else
+        load_tail(a, which, it.slot, it.h, 8 * th + i, q, w[i]);
+    }
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int pos = it.pg * kP + 8 * th + i;
-      // (rows of the page that this call does not bring come from the tail)
-      const int at = max(pos, it.s.start);
-      cache_row(a, which, it.s.first + at - it.s.start, it.h, at, q, w[i]);
-      if (pos < it.s.start) {
-        const uint16_t* tr = tail_row(a, which, it.slot, it.h, 8 * th + i);
-        const uint2 lo = *reinterpret_cast<const uint2*>(tr + 4 * q), hi = *reinterpret_cast<const uint2*>(tr + 64 + 4 * q);
-        w[i][0] = lo.x; w[i][1] = lo.y; w[i][2] = hi.x; w[i][3] = hi.y;
+      uint32_t f[4] = {w[i][0], w[i][1], w[i][2], w[i][3]};
+      cache_form<NORM>(a, which, pos, q, f);
+      if (pos >= it.s.start) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[i][j] = f[j];
       }
     }
     const int64_t page = static_cast<int64_t>(it.pool) * a.t.Hkv + it.h;
@@ -371,80 +448,91 @@ __global__ void __launch_bounds__(kRowWarps * 32) append_encode_kernel(const __g
                      static_cast<int64_t>(a.t.Hkv) * (kD / 2), a.base[which] + page * kD);
     if (lane == 0) a.rowmask[which][page] = static_cast<int32_t>(rm);
   } else if (it.pool >= 0 && !it.later) {
-    write_open(a, it, which, lane);
+    write_open<NORM>(a, it, which, lane);
   }
-  if (lane == 0) a.counts[static_cast<int64_t>(which) * a.items_pad + item] = static_cast<uint8_t>(__popc(rm));
+  if (lane == 0) {
+    const bool full = it.pool >= 0 && it.full;
+    a.counts[static_cast<int64_t>(which) * a.items_pad + item] =
+        static_cast<uint8_t>(__popc(rm) + (full ? kItemFull + (opens_later(it) ? kItemOpens : 0) : 0));
+    if (which == 0 && full) a.pages[item] = make_int2(it.pool * a.t.Hkv + it.h, it.s.b);
+  }
 }
 
-constexpr int kPlaceItems = 256;  // items of one CTA of append_place_kernel, one per thread
+constexpr int kPlaceItems = 64;     // items of one CTA of append_place_kernel
+constexpr int kPlaceThreads = 256;  // eight warps, eight items each
 
 // blockIdx.y: keys, values. The CTA adds up the counts of all items before its
-// own (bytes: 65,536 items are 16 loads of 16 bytes per thread), scans its
-// own, writes the offsets and copies the escaped rows.
-__global__ void __launch_bounds__(kPlaceItems) append_place_kernel(const __grid_constant__ Append a) {
-  __shared__ int s_warp[kPlaceItems / 32], s_before[kPlaceItems / 32];
-  __shared__ int s_off[kPlaceItems];
+// own (bytes: 65,536 items are 16 loads of 16 bytes per thread), scans its own,
+// writes the offsets and copies the escaped rows.
+template <bool NORM>
+__global__ void __launch_bounds__(kPlaceThreads) append_place_kernel(const __grid_constant__ Append a) {
+  __shared__ int s_before[kPlaceThreads / 32];
+  __shared__ int s_count[kPlaceItems], s_off[kPlaceItems];
   after_prior();
   const int which = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint8_t* counts = a.counts + static_cast<int64_t>(which) * a.items_pad;
   const int i0 = blockIdx.x * kPlaceItems, mine = i0 + threadIdx.x;
+  const int count = threadIdx.x < kPlaceItems && mine < a.items ? counts[mine] : 0;
+  const int2 page = threadIdx.x < kPlaceItems && (count & kItemFull) ? a.pages[mine] : make_int2(0, 0);
   int before = 0;
-  for (int i = threadIdx.x; i < i0 / 16; i += kPlaceItems) {
+  for (int i = threadIdx.x; i < i0 / 16; i += kPlaceThreads) {
     const uint4 v = reinterpret_cast<const uint4*>(counts)[i];
-    before = __dp4a(v.x, 0x01010101u, static_cast<uint32_t>(before));
-    before = __dp4a(v.y, 0x01010101u, static_cast<uint32_t>(before));
-    before = __dp4a(v.z, 0x01010101u, static_cast<uint32_t>(before));
-    before = __dp4a(v.w, 0x01010101u, static_cast<uint32_t>(before));
+    before = __dp4a(v.x & 0x1F1F1F1Fu, 0x01010101u, static_cast<uint32_t>(before));
+    before = __dp4a(v.y & 0x1F1F1F1Fu, 0x01010101u, static_cast<uint32_t>(before));
+    before = __dp4a(v.z & 0x1F1F1F1Fu, 0x01010101u, static_cast<uint32_t>(before));
+    before = __dp4a(v.w & 0x1F1F1F1Fu, 0x01010101u, static_cast<uint32_t>(before));
   }
-  const int n = mine < a.items ? counts[mine] : 0;
-  int incl = n;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xFFFFFFFFu, incl, d);
-    if (lane >= d) incl += y;
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, d);
-  if (lane == 31) s_warp[warp] = incl;
+  before = __reduce_add_sync(0xFFFFFFFFu, before);
   if (lane == 0) s_before[warp] = before;
+  if (threadIdx.x < kPlaceItems) s_count[threadIdx.x] = count;
   __syncthreads();
-  int off = a.base_cnt[which] + incl - n, total = 0;
-  for (int w = 0; w < kPlaceItems / 32; ++w) {
-    off += s_before[w];
-    if (w < warp) off += s_warp[w];
-    total += s_before[w] + s_warp[w];
+  if (threadIdx.x < kPlaceItems) {
+    int off = a.base_cnt[which], total = 0;
+    for (int w = 0; w < kPlaceThreads / 32; ++w) off += s_before[w];
+    for (int i = 0; i < kPlaceItems; ++i) {
+      const int n = s_count[i] & kItemRows;
+      off += i < threadIdx.x ? n : 0;
+      total += i >= threadIdx.x ? n : 0;
+    }
+    s_off[threadIdx.x] = off;
+    if (count & kItemFull) a.rowoff[which][page.x] = off;
+    // (may exceed the capacity: the caller grows the pool before it calls)
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *a.cnt[which] = off + total;
   }
-  s_off[threadIdx.x] = off;
-  // (may exceed the capacity: the caller grows the pool before it calls)
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *a.cnt[which] = a.base_cnt[which] + total;
   __syncthreads();
   const int q = lane & 15, th = lane >> 4;
-  for (int i = warp; i < kPlaceItems && i0 + i < a.items; i += kPlaceItems / 32) {
-    Item it = load_item(a, i0 + i, lane);
-    if (it.pool < 0 || !it.full) continue;
-    const int64_t page = static_cast<int64_t>(it.pool) * a.t.Hkv + it.h;
-    if (lane == 0) a.rowoff[which][page] = s_off[i];
-    uint32_t rm = static_cast<uint32_t>(a.rowmask[which][page]) & 0xFFFFu;
+  // the warp's eight items, every eighth of the CTA's (a sequence's heads, which
+  // have their open pages to write at once, go to different warps): those with
+  // escaped rows or an open page
+  constexpr int warps = kPlaceThreads / 32;
+  const int flags = lane < kPlaceItems / warps ? s_count[warps * lane + warp] : 0;
+  for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, (flags & (kItemRows | kItemOpens)) != 0); todo != 0u; todo &= todo - 1u) {
+    const int i = warps * (__ffs(todo) - 1) + warp, item = i0 + i;
+    const int2 at = a.pages[item];
+    Item it;
+    it.s = load_seq(a.t, at.y);
+    it.h = item % a.t.Hkv;
+    it.pg = it.s.start / kP + (a.t.cu_seqlens == nullptr ? 0 : item / a.t.Hkv - (it.s.first / kP + 2 * at.y));
+    it.slot = a.t.slots == nullptr ? at.y : __ldg(a.t.slots + at.y);
+    uint32_t rm = static_cast<uint32_t>(a.rowmask[which][at.x]) & 0xFFFFu;
     int64_t ridx = s_off[i];
     for (; rm != 0u; rm &= rm - 1u, ++ridx) {
       if (ridx < 0 || ridx >= a.cap[which]) continue;
       const int r = __ffs(rm) - 1, pos = it.pg * kP + r;
-      const int at = max(pos, it.s.start);
       uint32_t w[4];
-      cache_row(a, which, it.s.first + at - it.s.start, it.h, at, q, w);
       if (pos < it.s.start) {
-        const uint16_t* tr = tail_row(a, which, it.slot, it.h, r);
-        const uint2 lo = *reinterpret_cast<const uint2*>(tr + 4 * q), hi = *reinterpret_cast<const uint2*>(tr + 64 + 4 * q);
-        w[0] = lo.x; w[1] = lo.y; w[2] = hi.x; w[3] = hi.y;
+        load_tail(a, which, it.slot, it.h, r, q, w);
+      } else {
+        load_quads(a, which, it.s.first + pos - it.s.start, it.h, q, w);
+        cache_form<NORM>(a, which, pos, q, w);
       }
       if (th == 0) store_quads(a.raw[which] + ridx * kD, q, w);
     }
-    const int last = last_page(it.s);
-    if (it.pg == it.s.start / kP && it.s.start % kP != 0 && last > it.pg && (last + 1) * kP > it.s.start + it.s.n) {
-      it.pg = last;
-      it.pool = pool_page(a, it.s.b, last);
+    if (s_count[i] & kItemOpens) {
+      it.pg = last_page(it.s);
+      it.pool = pool_page(a, at.y, it.pg);
       __syncwarp();  // every lane has read the tail rows
-      if (it.pool >= 0) write_open(a, it, which, lane);
+      if (it.pool >= 0) write_open<NORM>(a, it, which, lane);
     }
   }
 }
@@ -461,7 +549,8 @@ int check_append(const exk_append* t) {
       t->seq_lens == nullptr || t->block_table == nullptr || (t->q_norm == nullptr) != (t->k_norm == nullptr))
     return EXK_EARG;
   if (t->N < 0 || t->B <= 0 || t->Hq <= 0 || t->Hkv <= 0 || t->Hq % t->Hkv != 0 || t->rope_rows <= 0 ||
-      t->max_pages <= 0 || t->max_pages > (1 << 26) || t->pool_pages <= 0)
+      t->max_pages <= 0 || t->max_pages > (1 << 26) || t->pool_pages <= 0 ||
+      static_cast<int64_t>(t->pool_pages) * t->Hkv >= (int64_t{1} << 31))
     return EXK_EARG;
   if (t->cu_seqlens == nullptr && t->N != t->B) return EXK_EARG;
   if (t->N > (1 << 28) || t->B > (1 << 24) || t->Hq > 4096) return EXK_EARG;
@@ -472,8 +561,19 @@ int check_append(const exk_append* t) {
   return 0;
 }
 
-int64_t row_blocks(const exk_append& t, int heads) {
-  const int64_t work = static_cast<int64_t>(t.N) * ((heads + 4 * kQuads - 1) / (4 * kQuads));
+// Steps of a warp of token_rows: one while the warps do not fill the GPU about
+// twice (short calls, where latency counts), else a whole token, so that the
+// look-up is paid once (11,016 tokens of 48 heads, two groups in flight: 50 us; one step
+// a warp: 68 us).
+int row_steps(const exk_append& t, int heads, int sms) {
+  const int quads = t.q_norm != nullptr ? kQuads<true> : kQuads<false>;
+  const int steps = (heads + 4 * quads - 1) / (4 * quads);
+  return static_cast<int64_t>(t.N) * steps > int64_t{48} * sms ? steps : 1;
+}
+
+int64_t row_blocks(const exk_append& t, int heads, int steps) {
+  const int quads = t.q_norm != nullptr ? kQuads<true> : kQuads<false>;
+  const int64_t work = static_cast<int64_t>(t.N) * ((heads + 4 * quads * steps - 1) / (4 * quads * steps));
   return (work + kRowWarps - 1) / kRowWarps;
 }
 
@@ -483,6 +583,8 @@ int64_t page_slots(const exk_append& t) {
 
 }  // namespace
 
+static_assert(sizeof(exk_append) == 184, "the Python binding packs these bytes");
+
 extern "C" int exk_rope_append_bf16(const exk_append* t, uint16_t* k_pool, uint16_t* v_pool, int32_t* status, int device,
                                     void* stream) {
   int r = check_append(t);
@@ -490,23 +592,26 @@ extern "C" int exk_rope_append_bf16(const exk_append* t, uint16_t* k_pool, uint1
   if (k_pool == nullptr || v_pool == nullptr) return EXK_EARG;
   if (!aligned16(k_pool) || !aligned16(v_pool)) return EXK_EALIGN;
   if (t->N == 0) return 0;
-  const int64_t blocks = row_blocks(*t, t->Hq + 2 * t->Hkv);
-  if (blocks >= (int64_t{1} << 31)) return EXK_EARG;
   DeviceScope scope;
-  if ((r = use_device(device, nullptr)) != 0) return r;
+  int sms = 0;
+  if ((r = use_device(device, &sms)) != 0) return r;
+  const int heads = t->Hq + 2 * t->Hkv, steps = row_steps(*t, heads, sms);
+  const int64_t blocks = row_blocks(*t, heads, steps);
+  if (blocks >= (int64_t{1} << 31)) return EXK_EARG;
   Append a = {};
   a.t = *t;
   a.pool[0] = k_pool;
   a.pool[1] = v_pool;
   a.status = status;
-  append_bf16_kernel<<<static_cast<unsigned>(blocks), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  const auto kernel = t->q_norm != nullptr ? append_bf16_kernel<true> : append_bf16_kernel<false>;
+  kernel<<<static_cast<unsigned>(blocks), kRowWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(a, steps);
   return launch_status();
 }
 
 extern "C" int64_t exk_rope_append_scratch(int N, int B, int Hkv, int packed) {
   if (N < 0 || B <= 0 || Hkv <= 0) return EXK_EARG;
   const int64_t items = (packed ? N / kP + 2 * static_cast<int64_t>(B) : B) * Hkv;
-  return 2 * ((items + 15) / 16 * 16) + 16;
+  return 16 + 2 * ((items + 15) / 16 * 16) + 8 * items;
 }
 
 extern "C" int exk_rope_append_compressed(const exk_append* t, const exk_cview* k, int64_t k_cap, int32_t* k_cnt,
@@ -545,30 +650,35 @@ extern "C" int exk_rope_append_compressed(const exk_append* t, const exk_cview* 
   if (scratch_bytes < exk_rope_append_scratch(t->N, t->B, t->Hkv, t->cu_seqlens != nullptr)) return EXK_EARG;
   if (t->N == 0) return 0;
   DeviceScope scope;
-  if ((r = use_device(device, nullptr)) != 0) return r;
+  int sms = 0;
+  if ((r = use_device(device, &sms)) != 0) return r;
   a.tails = static_cast<int32_t>(tails);
   a.slots = static_cast<int32_t>(page_slots(*t));
   a.items = static_cast<int32_t>(items);
   a.items_pad = static_cast<int32_t>((items + 15) / 16 * 16);
   a.base_cnt = static_cast<int32_t*>(scratch);
   a.counts = static_cast<uint8_t*>(scratch) + 16;
+  a.pages = reinterpret_cast<int2*>(a.counts + 2 * static_cast<int64_t>(a.items_pad));
   a.status = status;
   const int64_t enc = (2 * items + kRowWarps - 1) / kRowWarps;
-  const int64_t blocks = enc + row_blocks(*t, t->Hq);
+  const int steps = row_steps(*t, t->Hq, sms);
+  const int64_t blocks = enc + row_blocks(*t, t->Hq, steps);
   if (blocks >= (int64_t{1} << 31)) return EXK_EARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  append_encode_kernel<<<static_cast<unsigned>(blocks), kRowWarps * 32, 0, st>>>(a, static_cast<int>(enc));
+  const bool norm = t->q_norm != nullptr;
+  const auto encode = norm ? append_encode_kernel<true> : append_encode_kernel<false>;
+  encode<<<static_cast<unsigned>(blocks), kRowWarps * 32, 0, st>>>(a, static_cast<int>(enc), steps);
   if ((r = launch_status()) != 0) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((items + kPlaceItems - 1) / kPlaceItems), 2);
-  cfg.blockDim = dim3(kPlaceItems);
+  cfg.blockDim = dim3(kPlaceThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, append_place_kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, norm ? append_place_kernel<true> : append_place_kernel<false>, a);
   if (e == cudaSuccess) return 0;
   (void)cudaGetLastError();
   return static_cast<int>(e);

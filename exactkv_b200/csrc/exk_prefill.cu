@@ -13,6 +13,7 @@
 // MN-major as the TMA left it). Two 128-row tiles alternate, so the tensor
 // core works on one while the other's softmax runs.
 #include <algorithm>
+#include <atomic>
 
 #include "exk_device.cuh"
 #include "exk_encode.cuh"
@@ -138,27 +139,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
       : "memory");
 }
 
-// ---------------------------------------------------------------- two fp32 at once
-
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void split2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -518,6 +498,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* stop = &bars->stop;
 
+  allow_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->q_full[i], 1);
@@ -819,7 +800,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
 }
 
 // Partials of ns splits of each row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M),
-// 0 for a row without keys; rows of no sequence are left alone. One warp per row.
+// 0 for a row without keys; rows of no sequence are left alone. One warp per
+// row; a lane holds the weights of splits lane and lane + 32, and eight splits'
+// o are loaded before they are added, in split order.
+constexpr int kMaxSplits = 64;
+
 __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constant__ PrefillArgs a) {
   after_prior();
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -827,24 +812,42 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constan
   if (row >= static_cast<int64_t>(a.N) * a.Hq) return;
   const int tok = static_cast<int>(row / a.Hq);
   if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.B)) return;
-  const float* pm = a.pm + row * a.ns;
-  const float* pl = a.pl + row * a.ns;
-  float M = -INFINITY;
-  for (int s = lane; s < a.ns; s += 32) M = fmaxf(M, pm[s]);
+  float m[2], l[2], f[2];
+  float M = -INFINITY, den = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool in = lane + 32 * i < a.ns;
+    m[i] = in ? a.pm[row * a.ns + lane + 32 * i] : -INFINITY;
+    l[i] = in ? a.pl[row * a.ns + lane + 32 * i] : 0.f;
+    M = fmaxf(M, m[i]);
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
-  float den = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[i] = m[i] == -INFINITY ? (l[i] == 0.f ? 0.f : 1.f) : ex2(m[i] - M);  // (no key of the row: its o was not written)
+    den += f[i] * l[i];
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) den += __shfl_xor_sync(0xFFFFFFFFu, den, d);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < a.ns; ++s) {
-    const float ms = pm[s], ls = pl[s];
-    if (ms == -INFINITY && ls == 0.f) continue;  // the split holds no key of this row
-    const float f = M == -INFINITY ? 1.f : ex2(ms - M);
-    const float4 o = reinterpret_cast<const float4*>(a.po + (row * a.ns + s) * kD)[lane];
-    den += f * ls;
-    acc.x += f * o.x;
-    acc.y += f * o.y;
-    acc.z += f * o.z;
-    acc.w += f * o.w;
+  const float4* o = reinterpret_cast<const float4*>(a.po + row * a.ns * kD) + lane;
+  for (int s0 = 0; s0 < a.ns; s0 += 8) {
+    float4 v[8];
+    float g[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      g[u] = __shfl_sync(0xFFFFFFFFu, s0 < 32 ? f[0] : f[1], (s0 + u) & 31);
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + u < a.ns && g[u] != 0.f) v[u] = o[(s0 + u) * (kD / 4)];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      acc.x += g[u] * v[u].x;
+      acc.y += g[u] * v[u].y;
+      acc.z += g[u] * v[u].z;
+      acc.w += g[u] * v[u].w;
+    }
   }
   const float inv = den == 0.f ? 0.f : 1.f / den;
   uint16_t* d = a.out + tok * a.o_st + (row % a.Hq) * a.o_sh;
@@ -920,7 +923,7 @@ int64_t prefill_slots(int N, int B, int G) { return N / (2 * (kTile / G)) + stat
 
 int check_prefill(const exk_prefill* p) {
   if (p == nullptr || p->q == nullptr || p->out == nullptr || p->cu_q == nullptr) return EXK_EARG;
-  if (p->N < 0 || p->B <= 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv != 0 || p->ns < 1 || p->ns > 256 ||
+  if (p->N < 0 || p->B <= 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv != 0 || p->ns < 1 || p->ns > kMaxSplits ||
       p->N > (1 << 28) || p->B > (1 << 24) || p->Hq > 4096)
     return EXK_EARG;
   if (p->Hq / p->Hkv > 16) return EXK_EHEADS;
@@ -939,8 +942,21 @@ int make_rows_map(CUtensorMap* map, const uint16_t* p, int64_t rows, int heads, 
                       CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Lets the kernel have its shared memory, once per device (the current one).
+int allow_smem(int device) {
+  static std::atomic<uint64_t> done{0};
+  if (done.load(std::memory_order_acquire) >> device & 1) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrefillSmem);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return static_cast<int>(e);
+  }
+  done.fetch_or(uint64_t{1} << device, std::memory_order_release);
+  return 0;
+}
+
 int launch_prefill(const exk_prefill* p, PrefillArgs& a, const uint16_t* k, int64_t k_st, int64_t k_sh, const uint16_t* v,
-                   int64_t v_st, int64_t v_sh, int64_t key_rows, int key_box, int32_t* status, cudaStream_t st) {
+                   int64_t v_st, int64_t v_sh, int64_t key_rows, int key_box, int32_t* status, int device, cudaStream_t st) {
   if (!aligned16(k) || !aligned16(v)) return EXK_EALIGN;
   for (int64_t s : {k_st, k_sh, v_st, v_sh}) {
     if (s % 8 != 0) return EXK_EALIGN;
@@ -974,13 +990,23 @@ int launch_prefill(const exk_prefill* p, PrefillArgs& a, const uint16_t* k, int6
   if ((r = make_rows_map(&maps.q, p->q, p->N, p->Hq, p->q_st, p->q_sh, a.G, a.tpt)) != 0) return r;
   if ((r = make_rows_map(&maps.k, k, key_rows, p->Hkv, k_st, k_sh, 1, key_box)) != 0) return r;
   if ((r = make_rows_map(&maps.v, v, key_rows, p->Hkv, v_st, v_sh, 1, key_box)) != 0) return r;
-  const cudaError_t e = cudaFuncSetAttribute(prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrefillSmem);
-  if (e != cudaSuccess) return static_cast<int>(e);
+  if ((r = allow_smem(device)) != 0) return r;
   prefill_kernel<<<static_cast<unsigned>(grid), kPrefillThreads, kPrefillSmem, st>>>(a, maps);
   if ((r = launch_status()) != 0 || p->ns == 1) return r;
   const int64_t rows = static_cast<int64_t>(p->N) * p->Hq;
-  prefill_merge_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(a);
-  return launch_status();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t merge = cudaLaunchKernelEx(&cfg, prefill_merge_kernel, a);
+  if (merge == cudaSuccess) return 0;
+  (void)cudaGetLastError();
+  return static_cast<int>(merge);
 }
 
 }  // namespace
@@ -989,6 +1015,8 @@ int launch_prefill(const exk_prefill* p, PrefillArgs& a, const uint16_t* k, int6
 
 using namespace exk;
 
+static_assert(sizeof(exk_prefill) == 104, "the Python binding packs these bytes");
+
 extern "C" int exk_prefill_splits(int N, int B, int Hq, int Hkv, int64_t max_keys, int num_sms) {
   if (N < 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_keys < 0 || num_sms <= 0) return EXK_EARG;
   if (Hq / Hkv > 16) return EXK_EHEADS;
@@ -996,7 +1024,7 @@ extern "C" int exk_prefill_splits(int N, int B, int Hq, int Hkv, int64_t max_key
   const int64_t tiles = (max_keys + kTile - 1) / kTile;
   // whole waves of CTAs need no splits; else as many as fill the SMs once, of four key tiles at least
   const int64_t fit = items > 0 ? num_sms / items : 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({fit, tiles / 4, 64})));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({fit, tiles / 4, kMaxSplits})));
 }
 
 extern "C" int exk_attention_prefill(const exk_prefill* p, const uint16_t* k, int64_t k_st, int64_t k_sh,
@@ -1011,7 +1039,7 @@ extern "C" int exk_attention_prefill(const exk_prefill* p, const uint16_t* k, in
   PrefillArgs a = {};
   a.cu_k = cu_k;
   a.Nk = Nk;
-  return launch_prefill(p, a, k, k_st, k_sh, v, v_st, v_sh, Nk, kTile, status, static_cast<cudaStream_t>(stream));
+  return launch_prefill(p, a, k, k_st, k_sh, v, v_st, v_sh, Nk, kTile, status, device, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int exk_attention_prefill_paged(const exk_prefill* p, const uint16_t* k, const uint16_t* v, int pool_pages,
@@ -1031,7 +1059,7 @@ extern "C" int exk_attention_prefill_paged(const exk_prefill* p, const uint16_t*
   a.max_pages = max_pages;
   a.pool_pages = pool_pages;
   const int64_t st = static_cast<int64_t>(p->Hkv) * kD;
-  return launch_prefill(p, a, k, st, kD, v, st, kD, static_cast<int64_t>(pool_pages) * kP, kP, status,
+  return launch_prefill(p, a, k, st, kD, v, st, kD, static_cast<int64_t>(pool_pages) * kP, kP, status, device,
                         static_cast<cudaStream_t>(stream));
 }
 
@@ -1080,5 +1108,5 @@ extern "C" int exk_attention_prefill_paged_compressed(const exk_prefill* p, cons
   a.lens = seq_lens;
   a.k_stride = max_len;
   const int64_t st_e = static_cast<int64_t>(p->Hkv) * kD;
-  return launch_prefill(p, a, k_rows, st_e, kD, v_rows, st_e, kD, rows, kTile, status, st);
+  return launch_prefill(p, a, k_rows, st_e, kD, v_rows, st_e, kD, rows, kTile, status, device, st);
 }

@@ -23,7 +23,7 @@ import ctypes
 
 import torch
 
-from ._lib import Append, CView, Partials, Prefill, check, lib
+from ._lib import APPEND, CVIEW, PREFILL, CView, Partials, check, lib
 
 LOG2E = 1.4426950408889634
 P = 16          # tokens per page
@@ -501,82 +501,106 @@ def rope_table(inv_freq, positions, scale=1.0):
     return (torch.cat([ang.cos(), ang.sin()], 1) * scale).float()
 
 
-def _check_rows(t, name, n, heads=None):
-    """Strided token rows [n, heads, 128] of a packed batch."""
-    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != D or t.dtype != torch.bfloat16 or not t.is_cuda or \
-            t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be a CUDA bf16 tensor [N, heads, 128] with contiguous channels")
-    st, sh = t.stride(0), t.stride(1)
-    if st % 8 or sh % 8 or t.data_ptr() % 16 or st < 0 or sh <= 0 or (st == 0 and n > 1):
-        raise ValueError(f"{name}: token and head strides must be positive multiples of 8 elements, rows 16-byte aligned")
-    return st or t.shape[1] * D, sh
+def _stream(dev):
+    """The current stream of CUDA device number `dev` (torch.cuda.current_stream
+    builds an object for it, a tenth of a small call's time)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _check_index(t, name, shape, device):
-    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or t.shape != shape:
-        raise ValueError(f"{name} must be a contiguous int32 tensor {list(shape)} on {device}")
+def _rows(t, name, n, heads, dev):
+    """(address, token stride, head stride) of strided token rows [n, heads, 128] of a
+    packed batch on CUDA device `dev`, checked."""
+    shape, at = t.shape, t.data_ptr()
+    if len(shape) != 3 or shape[0] != n or shape[1] != heads or shape[2] != D or t.dtype is not torch.bfloat16 or \
+            t.device != dev or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA bf16 tensor [{n}, {heads}, {D}] on {dev}")
+    st, sh, sc = t.stride()
+    if sc != 1 or st % 8 or sh % 8 or at % 16 or st < 0 or sh <= 0 or (st == 0 and n > 1):
+        raise ValueError(f"{name}: channels must be contiguous, token and head strides positive multiples of 8 elements "
+                         "and rows 16-byte aligned")
+    return at, st or heads * D, sh
+
+
+def _index(t, name, shape, dev):
+    """Address of a contiguous int32 tensor of `shape` on `dev`, checked."""
+    if t.dtype is not torch.int32 or t.device != dev or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor {list(shape)} on {dev}")
     return t.data_ptr()
 
 
+def _heads(q, Hkv):
+    """(tokens, query heads) of packed queries, a multiple of Hkv."""
+    if q.dim() != 3 or q.shape[1] % Hkv:
+        raise ValueError(f"q must be [N, Hq, {D}] with Hq a multiple of the {Hkv} KV heads")
+    return q.shape[0], q.shape[1]
+
+
+def _new_rows(out, name, q, N, Hq):
+    """The output for q's rows: `out`, checked, or a new tensor, with its address and strides."""
+    if out is None:
+        out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=q.device)
+        return out, (out.data_ptr(), Hq * D, D)
+    return out, _rows(out, name, N, Hq, q.device)
+
+
 def _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, slots, q_norm, k_norm, eps, q_out, Hkv, pool_pages):
-    """exk_append of a call, checked, and its output."""
+    """exk_append of a call, checked; its output; tokens and sequences."""
     dev = q.device
-    N, Hq, _ = q.shape if q.dim() == 3 else (0, 0, 0)
-    q_st, q_sh = _check_rows(q, "q", N)
-    k_st, k_sh = _check_rows(k, "k", N, Hkv)
-    v_st, v_sh = _check_rows(v, "v", N, Hkv)
-    if Hq % Hkv:
-        raise ValueError(f"{Hq} query heads are no multiple of {Hkv} KV heads")
+    N, Hq = _heads(q, Hkv)
+    q_at, q_st, q_sh = _rows(q, "q", N, Hq, dev)
+    k_at, k_st, k_sh = _rows(k, "k", N, Hkv, dev)
+    v_at, v_st, v_sh = _rows(v, "v", N, Hkv, dev)
     if block_table.dim() != 2:
         raise ValueError("block_table must be [B, max_pages]")
     B, max_pages = block_table.shape
     if cu_seqlens is None and B != N:
         raise ValueError("without cu_seqlens every sequence brings one token: q must be [B, heads, 128]")
-    if cos_sin.dim() != 2 or cos_sin.shape[1] != D or cos_sin.dtype != torch.float32 or cos_sin.device != dev or \
+    if cos_sin.dim() != 2 or cos_sin.shape[1] != D or cos_sin.dtype is not torch.float32 or cos_sin.device != dev or \
             not cos_sin.is_contiguous():
-        raise ValueError(f"cos_sin must be a contiguous fp32 tensor [positions, 128] on {dev}")
-    if k.device != dev or v.device != dev:
-        raise ValueError("q, k and v must be on one device")
+        raise ValueError(f"cos_sin must be a contiguous fp32 tensor [positions, {D}] on {dev}")
     if (q_norm is None) != (k_norm is None):
         raise ValueError("q_norm and k_norm come together")
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None and (w.dtype != torch.bfloat16 or w.shape != (D,) or w.device != dev or not w.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous bf16 tensor [128] on {dev}")
-    if q_out is None:
-        q_out = torch.empty(N, Hq, D, dtype=q.dtype, device=dev)
-    elif q_out.device != dev:
-        raise ValueError("q_out must be on q's device")
-    o_st, o_sh = _check_rows(q_out, "q_out", N, Hq)
-    a = Append(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh,
-               cos_sin.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
-               None if k_norm is None else k_norm.data_ptr(),
-               None if cu_seqlens is None else _check_index(cu_seqlens, "cu_seqlens", (B + 1,), dev),
-               _check_index(seq_lens, "seq_lens", (B,), dev),
-               _check_index(block_table, "block_table", (B, max_pages), dev),
-               None if slots is None else _check_index(slots, "slots", (B,), dev),
-               N, B, Hq, Hkv, cos_sin.shape[0], max_pages, pool_pages, eps)
-    return a, q_out
+    wq = wk = 0
+    if q_norm is not None:
+        for w in (q_norm, k_norm):
+            if w.dtype is not torch.bfloat16 or w.shape != (D,) or w.device != dev or not w.is_contiguous():
+                raise ValueError(f"q_norm and k_norm must be contiguous bf16 tensors [{D}] on {dev}")
+        wq, wk = q_norm.data_ptr(), k_norm.data_ptr()
+    q_out, (o_at, o_st, o_sh) = _new_rows(q_out, "q_out", q, N, Hq)
+    a = APPEND.pack(q_at, k_at, v_at, o_at, q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, cos_sin.data_ptr(), wq, wk,
+                    0 if cu_seqlens is None else _index(cu_seqlens, "cu_seqlens", (B + 1,), dev),
+                    _index(seq_lens, "seq_lens", (B,), dev), _index(block_table, "block_table", (B, max_pages), dev),
+                    0 if slots is None else _index(slots, "slots", (B,), dev),
+                    N, B, Hq, Hkv, cos_sin.shape[0], max_pages, pool_pages, eps)
+    return a, q_out, N, B
 
 
 def _bf16_pool(k, v, q):
     """(KV heads, pages) of a pair of bf16 pools [B', TS', Hkv, 128]."""
-    for t in (k, v):
-        if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[3] != D or not t.is_contiguous() or t.shape != k.shape or \
-                t.device != q.device:
-            raise ValueError("k and v pools must be contiguous bf16 [B', TS', Hkv, 128] on q's device")
-    if k.shape[1] % P or k.numel() == 0:
+    shape, dev = k.shape, q.device
+    if len(shape) != 4 or shape[3] != D or v.shape != shape or k.dtype is not torch.bfloat16 or \
+            v.dtype is not torch.bfloat16 or k.device != dev or v.device != dev or \
+            not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("k and v pools must be contiguous bf16 [B', TS', Hkv, 128] on q's device")
+    B, TS, H, _ = shape
+    if TS % P or B * TS * H == 0:
         raise ValueError("a pool's TS' must be a positive multiple of 16")
-    return k.shape[2], k.shape[0] * k.shape[1] // P
+    return H, B * TS // P
 
 
-def _coded_pool(c, q, write):
-    """(exk_cview, KV heads, pages, slots of the raw pool, counter) of a cache used as a page pool."""
-    view, TS, H = _cache_args(c)
+def _coded_pool(c, dev, write):
+    """(exk_cview, KV heads, pages, slots of the raw pool, counter) of a cache used as a
+    page pool: a cache object, or a dict of its buffers."""
     if isinstance(c, dict):
-        B, sm, cap, cnt = c["shape"][0], c["sm"], c.get("cap"), c.get("cnt")
+        sm, raw, cap, cnt = c["sm"], c["raw"], c.get("cap"), c.get("cnt")
+        B, TS, H = c["shape"][:3]
+        view = CVIEW.pack(sm.data_ptr(), c["code"].data_ptr(), c["base"].data_ptr(), c["rowmask"].data_ptr(),
+                          c["rowoff"].data_ptr(), raw.data_ptr(), raw.shape[0])
     else:
+        view, TS, H = _cache_args(c)
+        view = ctypes.byref(view)
         B, sm, cap, cnt = c.B, c.sm, getattr(c, "cap", None), getattr(c, "cnt", None)
-    if sm.device != q.device:
+    if sm.device != dev:
         raise ValueError("the pools must be on q's device")
     if write and (cap is None or cnt is None):
         raise ValueError("a pool that is written needs its raw pool's capacity (cap) and counter (cnt)")
@@ -598,21 +622,21 @@ def rope_append_paged(q, k, v, cos_sin, kc, vc, block_table, seq_lens, cu_seqlen
     rows ahead (PagedCompressedKV.ensure_headroom(N)). Returns the rotated
     queries [N, Hq, 128] (q_out, which may be q). Positions or pages out of
     range are not stored and reported by check_status()."""
-    kv, H, pages, k_cap, k_cnt = _coded_pool(kc, q, True)
-    vv, vH, v_pages, v_cap, v_cnt = _coded_pool(vc, q, True)
+    kv, H, pages, k_cap, k_cnt = _coded_pool(kc, q.device, True)
+    vv, vH, v_pages, v_cap, v_cnt = _coded_pool(vc, q.device, True)
     if vH != H or v_pages != pages:
         raise ValueError("the key and value pools differ in shape")
-    a, q_out = _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, slots, q_norm, k_norm, eps, q_out, H,
-                            pages)
-    if a.N == 0:
+    a, q_out, N, B = _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, slots, q_norm, k_norm, eps, q_out,
+                                  H, pages)
+    if N == 0:
         return q_out
-    n = lib.exk_rope_append_scratch(a.N, a.B, H, cu_seqlens is not None)
+    n = lib.exk_rope_append_scratch(N, B, H, cu_seqlens is not None)
     scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
     dev = q.device.index
-    check(lib.exk_rope_append_compressed(ctypes.byref(a), ctypes.byref(kv), k_cap, k_cnt.data_ptr(), ctypes.byref(vv),
+    check(lib.exk_rope_append_compressed(a, kv, k_cap, k_cnt.data_ptr(), vv,
                                          v_cap, v_cnt.data_ptr(), scratch.data_ptr(), n,
                                          status_tensor(dev).data_ptr(), dev,
-                                         torch.cuda.current_stream(q.device).cuda_stream), "exk_rope_append_compressed")
+                                         _stream(dev)), "exk_rope_append_compressed")
     return q_out
 
 
@@ -621,47 +645,41 @@ def rope_append_reference_paged(q, k, v, cos_sin, k_pool, v_pool, block_table, s
     """The bf16 sibling of rope_append_paged over bf16 pools [B', TS', Hkv, 128]
     (pages of 16 rows): the same values in the same places."""
     H, pages = _bf16_pool(k_pool, v_pool, q)
-    a, q_out = _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, None, q_norm, k_norm, eps, q_out, H,
-                            pages)
-    if a.N == 0:
+    a, q_out, N, _ = _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, None, q_norm, k_norm, eps, q_out,
+                                  H, pages)
+    if N == 0:
         return q_out
     dev = q.device.index
-    check(lib.exk_rope_append_bf16(ctypes.byref(a), k_pool.data_ptr(), v_pool.data_ptr(), status_tensor(dev).data_ptr(),
-                                   dev, torch.cuda.current_stream(q.device).cuda_stream), "exk_rope_append_bf16")
+    check(lib.exk_rope_append_bf16(a, k_pool.data_ptr(), v_pool.data_ptr(), status_tensor(dev).data_ptr(),
+                                   dev, _stream(dev)), "exk_rope_append_bf16")
     return q_out
 
 
 # ----------------------------------------------------------------------------- prompt attention
 
 def _prefill_args(q, cu_seqlens, Hkv, max_keys, out):
-    """exk_prefill of a call, checked, its output, and the workspace it names. The
-    workspace belongs to the call (inside a capture: to the graph), so no two
-    calls share it."""
+    """exk_prefill of a call, checked; its output; tokens and sequences; and the
+    workspace it names, which belongs to the call (inside a capture: to the
+    graph), so no two calls share it."""
     dev = q.device
-    N, Hq, _ = q.shape if q.dim() == 3 else (0, 0, 0)
-    q_st, q_sh = _check_rows(q, "q", N)
-    if Hq % Hkv:
-        raise ValueError(f"{Hq} query heads are no multiple of {Hkv} KV heads")
+    N, Hq = _heads(q, Hkv)
+    q_at, q_st, q_sh = _rows(q, "q", N, Hq, dev)
     B = cu_seqlens.numel() - 1
     if B < 1:
         raise ValueError("cu_seqlens must hold B + 1 offsets")
-    cu = _check_index(cu_seqlens, "cu_seqlens", (B + 1,), dev)
-    if out is None:
-        out = torch.empty(N, Hq, D, dtype=q.dtype, device=dev)
-    elif out.device != dev:
-        raise ValueError("out must be on q's device")
-    o_st, o_sh = _check_rows(out, "out", N, Hq)
+    cu = _index(cu_seqlens, "cu_seqlens", (B + 1,), dev)
+    out, (o_at, o_st, o_sh) = _new_rows(out, "out", q, N, Hq)
     ns = lib.exk_prefill_splits(N, B, Hq, Hkv, max_keys, num_sms(dev.index))
     if ns < 0:
         check(ns, "exk_prefill_splits")
-    ws, o, m, l = None, None, None, None
+    ws, o, m, l = None, 0, 0, 0
     if ns > 1:
         rows = N * Hq * ns
         ws = torch.empty(rows * (D + 2), dtype=torch.float32, device=dev)
         o = ws.data_ptr()
         m, l = o + rows * D * 4, o + rows * (D + 1) * 4
-    return Prefill(q.data_ptr(), out.data_ptr(), q_st, q_sh, o_st, o_sh, cu, o, m, l, N, B, Hq, Hkv, ns,
-                   D ** -0.5 * LOG2E), out, ws
+    a = PREFILL.pack(q_at, o_at, q_st, q_sh, o_st, o_sh, cu, o, m, l, N, B, Hq, Hkv, ns, D ** -0.5 * LOG2E)
+    return a, out, N, B, ws
 
 
 def attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None):
@@ -673,26 +691,24 @@ def attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None):
     excess as context; a query that sees no key gives zeros. Up to 16 query
     heads per KV head. Returns bf16 [N, Hq, 128]; rows past cu_seqlens[B] are
     left as they were."""
-    if k.dim() != 3 or k.device != q.device or v.device != q.device:
-        raise ValueError("k and v must be [Nk, Hkv, 128] on q's device")
-    Nk, Hkv, _ = k.shape
-    if Nk == 0 or Hkv == 0:
-        raise ValueError("k and v must hold at least one row")
-    k_st, k_sh = _check_rows(k, "k", Nk)
-    v_st, v_sh = _check_rows(v, "v", Nk, Hkv)
-    a, out, ws = _prefill_args(q, cu_seqlens, Hkv, Nk, out)
+    if k.dim() != 3 or k.shape[0] == 0 or k.shape[1] == 0:
+        raise ValueError("k and v must be [Nk, Hkv, 128] with at least one row")
+    Nk, Hkv = k.shape[:2]
+    k_at, k_st, k_sh = _rows(k, "k", Nk, Hkv, q.device)
+    v_at, v_st, v_sh = _rows(v, "v", Nk, Hkv, q.device)
+    a, out, N, B, ws = _prefill_args(q, cu_seqlens, Hkv, Nk, out)
     if cu_seqlens_k is None:
-        if Nk != a.N:
+        if Nk != N:
             raise ValueError("k and v rows differ from q's: give cu_seqlens_k")
-        cu_k = a.cu_q
+        cu_k = cu_seqlens.data_ptr()
     else:
-        cu_k = _check_index(cu_seqlens_k, "cu_seqlens_k", (a.B + 1,), q.device)
-    if a.N == 0:
+        cu_k = _index(cu_seqlens_k, "cu_seqlens_k", (B + 1,), q.device)
+    if N == 0:
         return out
     dev = q.device.index
-    check(lib.exk_attention_prefill(ctypes.byref(a), k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, Nk, cu_k,
+    check(lib.exk_attention_prefill(a, k_at, k_st, k_sh, v_at, v_st, v_sh, Nk, cu_k,
                                     status_tensor(dev).data_ptr(), dev,
-                                    torch.cuda.current_stream(q.device).cuda_stream), "exk_attention_prefill")
+                                    _stream(dev)), "exk_attention_prefill")
     return out
 
 
@@ -709,8 +725,8 @@ def _most_keys(block_table, max_len):
 
 def _check_pages(block_table, seq_lens, B, dev):
     max_pages = block_table.shape[1]
-    return (_check_index(block_table, "block_table", (B, max_pages), dev), max_pages,
-            _check_index(seq_lens, "seq_lens", (B,), dev))
+    return (_index(block_table, "block_table", (B, max_pages), dev), max_pages,
+            _index(seq_lens, "seq_lens", (B,), dev))
 
 
 def attention_prefill_paged(q, kc, vc, block_table, seq_lens, cu_seqlens, max_len=None, out=None):
@@ -720,21 +736,21 @@ def attention_prefill_paged(q, kc, vc, block_table, seq_lens, cu_seqlens, max_le
     them. max_len (host, at least every seq_lens[b]; default max_pages * 16)
     bounds the workspace of B * max_len decoded rows. Bit-identical to
     attention_prefill_reference_paged for the same values and max_len."""
-    kv, H, pages, _, _ = _coded_pool(kc, q, False)
-    vv, vH, v_pages, _, _ = _coded_pool(vc, q, False)
+    kv, H, pages, _, _ = _coded_pool(kc, q.device, False)
+    vv, vH, v_pages, _, _ = _coded_pool(vc, q.device, False)
     if vH != H or v_pages != pages:
         raise ValueError("the key and value pools differ in shape")
     rows = _most_keys(block_table, max_len)
-    a, out, ws = _prefill_args(q, cu_seqlens, H, rows, out)
-    table, max_pages, lens = _check_pages(block_table, seq_lens, a.B, q.device)
-    if a.N == 0:
+    a, out, N, B, ws = _prefill_args(q, cu_seqlens, H, rows, out)
+    table, max_pages, lens = _check_pages(block_table, seq_lens, B, q.device)
+    if N == 0:
         return out
-    kv_rows = torch.empty(2, a.B * rows, H, D, dtype=torch.bfloat16, device=q.device)
+    kv_rows = torch.empty(2, B * rows, H, D, dtype=torch.bfloat16, device=q.device)
     dev = q.device.index
     check(lib.exk_attention_prefill_paged_compressed(
-        ctypes.byref(a), ctypes.byref(kv), ctypes.byref(vv), pages, table, max_pages, lens, kv_rows[0].data_ptr(),
+        a, kv, vv, pages, table, max_pages, lens, kv_rows[0].data_ptr(),
         kv_rows[1].data_ptr(), rows, status_tensor(dev).data_ptr(), dev,
-        torch.cuda.current_stream(q.device).cuda_stream), "exk_attention_prefill_paged_compressed")
+        _stream(dev)), "exk_attention_prefill_paged_compressed")
     return out
 
 
@@ -743,13 +759,13 @@ def attention_prefill_reference_paged(q, k, v, block_table, seq_lens, cu_seqlens
     Hkv, 128] (pages of 16 rows), read in place: no workspace of rows, and max_len
     only bounds the plan of the splits."""
     H, pages = _bf16_pool(k, v, q)
-    a, out, ws = _prefill_args(q, cu_seqlens, H, _most_keys(block_table, max_len), out)
-    table, max_pages, lens = _check_pages(block_table, seq_lens, a.B, q.device)
-    if a.N == 0:
+    a, out, N, B, ws = _prefill_args(q, cu_seqlens, H, _most_keys(block_table, max_len), out)
+    table, max_pages, lens = _check_pages(block_table, seq_lens, B, q.device)
+    if N == 0:
         return out
     dev = q.device.index
-    check(lib.exk_attention_prefill_paged(ctypes.byref(a), k.data_ptr(), v.data_ptr(), pages, table, max_pages, lens,
+    check(lib.exk_attention_prefill_paged(a, k.data_ptr(), v.data_ptr(), pages, table, max_pages, lens,
                                           status_tensor(dev).data_ptr(), dev,
-                                          torch.cuda.current_stream(q.device).cuda_stream),
+                                          _stream(dev)),
           "exk_attention_prefill_paged")
     return out

@@ -423,15 +423,15 @@ def test_refusals():
 def test_entry_points_refuse_before_any_launch():
     """Argument errors of the C entries come back as codes (addresses never touched)."""
     import ctypes
-    from exactkv_b200._lib import Append, CView, Prefill, lib
+    from exactkv_b200._lib import APPEND, PREFILL, CView, lib
     at = 1 << 40
+    names = ("q k v q_out q_st q_sh k_st k_sh v_st v_sh o_st o_sh cos_sin q_norm k_norm cu_seqlens seq_lens block_table "
+             "slots N B Hq Hkv rope_rows max_pages pool_pages eps").split()
+    fits = dict(zip(names, (at, at, at, at, 1024, 128, 256, 128, 256, 128, 1024, 128, at, 0, 0, 0, at, at, 0, 4, 4, 8, 2,
+                            64, 4, 16, 1e-6)))
 
     def app(**kw):
-        a = Append(at, at, at, at, 1024, 128, 256, 128, 256, 128, 1024, 128, at, None, None, None, at, at, None, 4, 4, 8,
-                   2, 64, 4, 16, 1e-6)
-        for n, v in kw.items():
-            setattr(a, n, v)
-        return ctypes.byref(a)
+        return APPEND.pack(*{**fits, **{n: v or 0 for n, v in kw.items()}}.values())
 
     bf = lambda a, k=at: lib.exk_rope_append_bf16(a, k, at, None, 0, None)  # noqa: E731
     assert lib.exk_rope_append_bf16(None, at, at, None, 0, None) == -1
@@ -450,11 +450,12 @@ def test_entry_points_refuse_before_any_launch():
     assert coded(bytes_=n - 1) == -1 and coded(k=short) == -1 and coded(cap=-1) == -1 and coded(scratch=None) == -1
     assert coded(scratch=at + 4) == -2 and coded(a=app(Hq=7)) == -1
 
+    pnames = "q out q_st q_sh o_st o_sh cu_q po pm pl N B Hq Hkv ns qk_scale".split()
+    pfits = dict(zip(pnames, (at, at, 1024, 128, 1024, 128, at, 0, 0, 0, 4, 1, 8, 2, 1, 0.1)))
+
     def pre(**kw):
-        p = Prefill(at, at, 1024, 128, 1024, 128, at, None, None, None, 4, 1, 8, 2, 1, 0.1)
-        for name, v in kw.items():
-            setattr(p, name, v)
-        return lib.exk_attention_prefill(ctypes.byref(p), at, 256, 128, at, 256, 128, 4, at, None, 0, None)
+        p = PREFILL.pack(*{**pfits, **{n: v or 0 for n, v in kw.items()}}.values())
+        return lib.exk_attention_prefill(p, at, 256, 128, at, 256, 128, 4, at, None, 0, None)
 
     for kw in (dict(q=None), dict(B=0), dict(Hq=7), dict(ns=0), dict(ns=2), dict(q_st=0), dict(cu_q=None)):
         assert pre(**kw) == -1, kw
