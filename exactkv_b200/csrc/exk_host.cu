@@ -45,6 +45,24 @@ int make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* ptr, u
   return r == CUDA_SUCCESS ? 0 : EXK_ETMAP;
 }
 
+int make_tmap(CUtensorMap* map, CUtensorMapDataType dtype, const void* ptr, int rank, const uint64_t* dims,
+              const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return EXK_EDRIVER;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    estr[i] = 1;
+    if (i > 0) st[i - 1] = strides[i - 1];
+  }
+  CUresult r = fn(map, dtype, static_cast<cuuint32_t>(rank), const_cast<void*>(ptr), d, st, b, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : EXK_ETMAP;
+}
+
 int use_device(int device, int* num_sms) {
   if (device < 0 || device >= kMaxDevices) return EXK_EARG;
   cudaError_t e = cudaSetDevice(device);

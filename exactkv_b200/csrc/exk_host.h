@@ -14,6 +14,11 @@ int make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* ptr, u
                  uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0, uint32_t box1,
                  uint32_t box2, CUtensorMapSwizzle swizzle);
 
+// The same for `rank` dimensions (at most 5): dims and box [rank], strides of
+// dimensions 1 .. rank - 1 in bytes.
+int make_tmap(CUtensorMap* map, CUtensorMapDataType dtype, const void* ptr, int rank, const uint64_t* dims,
+              const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle);
+
 // Makes `device` current for this library's runtime (the caller's framework
 // keeps its own notion of the current device) and returns its SM count.
 int use_device(int device, int* num_sms);

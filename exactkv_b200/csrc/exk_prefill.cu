@@ -52,6 +52,7 @@ struct PrefillArgs {
   int32_t* status;
   int N, Nk, B, Hq, Hkv, G, tpt;  // tpt: tokens of a query tile
   int max_pages, pool_pages, ns, slots;
+  uint64_t by_block;           // divides by the tokens of a block (divide())
   float scale;                 // log2(e) / sqrt(128)
 };
 
@@ -172,17 +173,18 @@ __device__ __forceinline__ void steal_block(void* answer, uint64_t* bar) {
                "r"(smem_addr(bar))
                : "memory");
 }
-// The block taken, or -1: none was left.
-__device__ __forceinline__ int stolen_block(const void* answer) {
-  int x;
+// The block taken, or (-1, 0): none was left.
+__device__ __forceinline__ int2 stolen_block(const void* answer) {
+  int2 at;
   asm volatile(
-      "{\n .reg .b128 h;\n .reg .pred p;\n ld.shared.b128 h, [%1];\n mov.b32 %0, -1;\n"
+      "{\n .reg .b128 h;\n .reg .pred p;\n ld.shared.b128 h, [%2];\n mov.b32 %0, -1;\n mov.b32 %1, 0;\n"
       " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
-      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n}"
-      : "=r"(x)
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::y.b32.b128 %1, h;\n}"
+      : "=r"(at.x), "=r"(at.y)
       : "r"(smem_addr(answer))
       : "memory");
-  return x;
+  return at;
 }
 
 struct Work {
@@ -197,19 +199,26 @@ struct Work {
   int masked;       // the first of the tiles, in which some row does not see some key
 };
 
-// Item `item` of the grid: (256-row block, KV head, split). Sequence b's blocks take
-// slots cu[b] / T + b, + 1, ... with T = 2 tpt tokens a block: n tokens need
-// at most (n + T - 1) / T, which never reaches sequence b + 1's first slot.
-// False for a slot left over. By a whole warp.
-__device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int lane, Work& w) {
+// x / T for 0 <= x < 2^28, T <= 256, with m = 2^36 / T + 1.
+__device__ __forceinline__ int divide(int x, uint64_t m) { return static_cast<int>((static_cast<uint64_t>(x) * m) >> 36); }
+
+// Block (x, y) of the grid: (KV head, split) and 256-row block, long rows of keys
+// first. Sequence b's blocks take slots cu[b] / T + b, + 1, ... with T = 2 tpt
+// tokens a block: n tokens need at most (n + T - 1) / T, which never reaches
+// sequence b + 1's first slot. False for a slot left over. By a whole warp.
+__device__ __forceinline__ bool load_work(const PrefillArgs& a, int2 block, int lane, Work& w) {
+  if (block.x < 0) return false;
   const int T = 2 * a.tpt;
-  if (item < 0) return false;
-  w.split = item % a.ns;
-  w.hk = (item / a.ns) % a.Hkv;
-  const int slot = a.slots - 1 - item / (a.ns * a.Hkv);  // long rows of keys first
+  w.split = 0;
+  w.hk = block.x;
+  if (a.ns > 1) {
+    w.hk = block.x / a.ns;
+    w.split = block.x - w.hk * a.ns;
+  }
+  const int slot = a.slots - 1 - block.y;
   int b = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const bool before = b0 + lane < a.B && __ldg(a.cu_q + b0 + lane + 1) / T + b0 + lane + 1 <= slot;
+    const bool before = b0 + lane < a.B && divide(__ldg(a.cu_q + b0 + lane + 1), a.by_block) + b0 + lane + 1 <= slot;
     b += __popc(__ballot_sync(0xFFFFFFFFu, before));
   }
   if (b >= a.B) return false;
@@ -218,7 +227,7 @@ __device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int la
   w.first = __ldg(a.cu_q + b);
   w.n = __ldg(a.cu_q + b + 1) - w.first;
   if (w.first < 0 || w.n <= 0 || w.first > a.N - w.n) return false;
-  w.tok0 = (slot - (w.first / T + b)) * T;
+  w.tok0 = (slot - (divide(w.first, a.by_block) + b)) * T;
   if (w.tok0 < 0 || w.tok0 >= w.n) return false;
   if (a.cu_k != nullptr) {
     w.krow = __ldg(a.cu_k + b);
@@ -233,7 +242,7 @@ __device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int la
   w.tiles = w.n - w.tok0 > a.tpt ? 2 : 1;
   w.keys = max(0, w.L - w.n + min(w.tok0 + T, w.n));
   const int all = (w.keys + kTile - 1) / kTile;
-  const int per = (all + a.ns - 1) / a.ns;
+  const int per = a.ns > 1 ? (all + a.ns - 1) / a.ns : all;
   const int t0 = min(all, w.split * per);
   w.t1 = min(all, t0 + per);
   w.nt = w.t1 - t0;
@@ -243,16 +252,21 @@ __device__ __forceinline__ bool load_work(const PrefillArgs& a, int item, int la
   return true;
 }
 
-// Waits that end: after kWaitLimitNs, or at once when another role gave up.
+// Waits that end: after about two seconds, or at once when another role gave up.
+// The cycle counter rather than %globaltimer keeps the loop small: this
+// kernel's roles share the instruction cache, and at the change of an item all
+// of them run code that the main loop does not.
+constexpr uint32_t kWaitCycles = 3500000000u;  // 1.8 s at 1.965 GHz
+__device__ __forceinline__ uint32_t cycles() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
+  return t;
+}
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer();
+  const uint32_t t0 = cycles();
   while (!mbar_try_wait(bar, parity)) {
+    if (cycles() - t0 > kWaitCycles) *stop = 1;
     if (*stop != 0) return false;
-    if (globaltimer() - t0 > kWaitLimitNs) {
-      *stop = 1;
-      return false;
-    }
   }
   return true;
 }
@@ -265,6 +279,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 // Bits 15 and 31: the half's exponent field is all ones.
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+}
+
+// f += the values of v [32] that are not finite.
+__device__ __forceinline__ void add_not_finite(float (&f)[32], const uint4* v) {
+  uint32_t any = 0u;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) any |= not_finite(v[i].x) | not_finite(v[i].y) | not_finite(v[i].z) | not_finite(v[i].w);
+  if (any == 0u) return;
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(v);
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if ((h[i] & 0x7F80) == 0x7F80) f[i] += __uint_as_float(static_cast<uint32_t>(h[i]) << 16);
 }
 
 struct __align__(16) Bars {
@@ -282,14 +308,15 @@ constexpr int kStage = 4 * 2 * 32 * 128;
 constexpr int kPrefillSmem = 2 * kOperand + kSlots * kOperand + kStage + static_cast<int>(sizeof(Bars)) + 1024;
 static_assert(kPrefillSmem <= 227 * 1024, "one CTA's shared memory");
 
-// The softmax threads' side of one item: query tile x, a row per thread. s_phase:
+// The softmax threads' side of one item: query tile x, a row per thread; rt: the
+// row's token in the tile. s_phase:
 // tiles of S this thread has taken so far.
-__device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w, Bars* bars, uint32_t tmem, int x,
+__device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w, Bars* bars, uint32_t tmem, int x, int rt,
                                              uint32_t& s_phase, uint32_t& o_phase, volatile int* stop) {
   const int warp = threadIdx.x >> 5, r = threadIdx.x & 127;
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
   const uint32_t ts = tmem + lanes + x * kTile, to = tmem + lanes + 2 * kTile + x * kTile;
-  const int tok = w.tok0 + x * a.tpt + r / a.G;
+  const int tok = w.tok0 + x * a.tpt + rt;
   const bool valid = r < a.G * a.tpt && tok < w.n;
   const int lim = valid ? w.L - w.n + tok : w.keys - 1;  // last key the row sees
   const int nt = w.nt;
@@ -303,8 +330,8 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
     for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
     tc_wait_ld();
     if (it < w.masked) {
-      // columns past the last key the row sees; groups of 32 that every row of the
-      // warp sees are left alone
+      // columns past the last key that the row sees; groups of 32 that every row
+      // of the warp sees are left alone
       const int seen = lim - (w.t1 - 1 - it) * kTile;
       const int least = __reduce_min_sync(0xFFFFFFFFu, seen);
 #pragma unroll
@@ -375,7 +402,7 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
     bars->l[x][r] = l;
     mbar_arrive(&bars->l_full[x]);
     if (a.ns > 1 && valid) {
-      const int64_t at = (static_cast<int64_t>(w.first + tok) * a.Hq + w.hk * a.G + r % a.G) * a.ns + w.split;
+      const int64_t at = (static_cast<int64_t>(w.first + tok) * a.Hq + w.hk * a.G + r - rt * a.G) * a.ns + w.split;
       a.pm[at] = m;
       a.pl[at] = l;
     }
@@ -384,11 +411,11 @@ __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w
 }
 
 // The output warps' side of query tile x: row r = TMEM lane, thread r of the four warps.
-__device__ __forceinline__ void output_item(const PrefillArgs& a, const Work& w, Bars* bars, uint4* stage, uint32_t tmem, int x,
+__device__ __forceinline__ void output_item(const PrefillArgs& a, const Work& w, Bars* bars, uint4* stage, uint32_t tmem, int x, int rt,
                                             uint32_t& o_phase, volatile int* stop) {
   const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, r = threadIdx.x & 127;
   const uint32_t to = tmem + (static_cast<uint32_t>(warp) << 21) + 2 * kTile + x * kTile;
-  const int g = r % a.G, tok = w.tok0 + x * a.tpt + r / a.G;
+  const int g = r - rt * a.G, tok = w.tok0 + x * a.tpt + rt;
   const bool valid = r < a.G * a.tpt && tok < w.n;
   const int lim = w.L - w.n + tok;
   const int h = w.hk * a.G + g;
@@ -422,7 +449,7 @@ __device__ __forceinline__ void output_item(const PrefillArgs& a, const Work& w,
   // own threads, 16 bytes a row, the tile took 6,000 cycles.
   uint4* mine = stage + warp * 512;
   auto flush = [&](int part) {
-#pragma unroll
+#pragma unroll 4
     for (int i = 0; i < 8; ++i) {
       const int from = 4 * i + (lane >> 3);
       const uint64_t d = __shfl_sync(0xFFFFFFFFu, dst, from);
@@ -443,6 +470,7 @@ __device__ __forceinline__ void output_item(const PrefillArgs& a, const Work& w,
     if (bad && valid) {
       // a masked tile held values that are not finite: they were left out of
       // the product and reach the rows that see them here
+#pragma unroll 1
       for (int t = max(w.low, (w.t1 - w.nt) * kTile); t < min(w.t1 * kTile, lim + 1); ++t) {
         int64_t vrow = static_cast<int64_t>(w.krow) + t;
         if (a.block_table != nullptr) {
@@ -450,10 +478,7 @@ __device__ __forceinline__ void output_item(const PrefillArgs& a, const Work& w,
           if (pg < 0 || pg >= a.pool_pages) continue;
           vrow = static_cast<int64_t>(pg) * kP + t % kP;
         }
-        const uint16_t* vp = a.v + vrow * a.v_st + w.hk * a.v_sh + 32 * c;
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if ((vp[i] & 0x7F80) == 0x7F80) f[i] += __uint_as_float(static_cast<uint32_t>(vp[i]) << 16);
+        add_not_finite(f, reinterpret_cast<const uint4*>(a.v + vrow * a.v_st + w.hk * a.v_sh + 32 * c));
       }
     }
     if (a.ns > 1) {
@@ -478,8 +503,8 @@ __device__ __forceinline__ void output_item(const PrefillArgs& a, const Work& w,
   }
   if (a.ns == 1) {
     __syncwarp();
-    flush(0);
-    flush(1);
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) flush(part);
   }
   __syncwarp();
 }
@@ -542,17 +567,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    const int x = warp >> 2;
+    const int x = warp >> 2, rt = (threadIdx.x & 127) / a.G;
     uint32_t s_phase = 0, o_phase = 0;
     Work w;
     while (next_work(w))
-      if (x < w.tiles) softmax_item(a, w, bars, tmem, x, s_phase, o_phase, stop);
+      if (x < w.tiles) softmax_item(a, w, bars, tmem, x, rt, s_phase, o_phase, stop);
   } else if (warp < kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOutput));
+    const int rt = (threadIdx.x & 127) / a.G;
     uint32_t o_phase = 0;
     Work w;
     while (next_work(w))
-      for (int x = 0; x < w.tiles; ++x) output_item(a, w, bars, stage, tmem, x, o_phase, stop);
+      for (int x = 0; x < w.tiles; ++x) output_item(a, w, bars, stage, tmem, x, rt, o_phase, stop);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == kMmaWarp) {
@@ -634,10 +660,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (!ok) break;
       }
     } else if (warp == kTmaWarp) {
-      // ---- TMA
-      const int tile_bytes = 64 * 2 * a.G * a.tpt;
+      // ---- TMA: an item's first K, its queries, its V, K, V, ...
+      const uint32_t tile_bytes = 2 * 64 * 2 * a.G * a.tpt;
       uint32_t e = 0, q_phase = 3;
-      if (lane == 0) {
+      if (elect_one()) {
         prefetch_tmap(&maps.q);
         prefetch_tmap(&maps.k);
         prefetch_tmap(&maps.v);
@@ -645,16 +671,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       Work w;
       while (next_work(w)) {
         bool ok = true;
-        for (int x = 0; w.nt > 0 && x < w.tiles && ok; ++x) {
-          ok = warp_wait(&bars->q_empty[x], (q_phase >> x) & 1, stop);
-          q_phase ^= 1u << x;
-          if (ok && lane == 0) {
-            mbar_arrive_expect_tx(&bars->q_full[x], 2 * tile_bytes);
-            for (int c = 0; c < 2; ++c)
-              tma_load_3d(sq + x * kOperand + c * kHalf, &maps.q, 64 * c, w.hk * a.G, w.first + w.tok0 + x * a.tpt,
-                          &bars->q_full[x]);
-          }
-        }
         for (int i = 0; i < 2 * w.nt && ok; ++i, ++e) {
           const uint32_t slot = e % kSlots;
           const int j = w.t1 - 1 - i / 2;
@@ -662,33 +678,42 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           if (!ok) break;
           const CUtensorMap* map = (i & 1) == 0 ? &maps.k : &maps.v;
           uint8_t* dst = ring + slot * kOperand;
+          uint64_t* full = &bars->kv_full[slot];
           if (a.block_table == nullptr) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&bars->kv_full[slot], kOperand);
-              for (int c = 0; c < 2; ++c)
-                tma_load_3d(dst + c * kHalf, map, 64 * c, w.hk, w.krow + j * kTile, &bars->kv_full[slot]);
+            if (elect_one()) {
+              mbar_arrive_expect_tx(full, kOperand);
+              tma_load_4d(dst, map, 0, w.hk, w.krow + j * kTile, 0, full);
             }
           } else {
-            // one lane per page; pages past the keys are not loaded (their columns are masked)
-            const int pages = min(kTile / kP, (w.keys - j * kTile + kP - 1) / kP);
+            // one lane per half page; pages past the keys are not loaded (their columns are masked)
+            const int pages = min(kTile / kP, (w.keys - j * kTile + kP - 1) / kP), pg = lane >> 1;
             int row = 0;
-            if (lane < pages) {
-              const int pg = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + j * (kTile / kP) + lane);
-              if (pg >= 0 && pg < a.pool_pages) {
-                row = pg * kP;
+            if (pg < pages) {
+              const int page = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + j * (kTile / kP) + pg);
+              if (page >= 0 && page < a.pool_pages) {
+                row = page * kP;
               } else {
                 set_status(a.status, EXK_S_PAGE_INDEX);
                 row = a.pool_pages * kP;  // outside the map: zeros
               }
             }
-            if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[slot], pages * (2 * 64 * 2 * kP));
+            if (lane == 0) mbar_arrive_expect_tx(full, pages * (2 * 64 * 2 * kP));
             __syncwarp();
-            if (lane < pages) {
-              for (int c = 0; c < 2; ++c)
-                tma_load_3d(dst + c * kHalf + lane * (kP * 128), map, 64 * c, w.hk, row, &bars->kv_full[slot]);
-            }
+            if (pg < pages) tma_load_4d(dst + (lane & 1) * kHalf + pg * (kP * 128), map, 0, w.hk, row, lane & 1, full);
           }
           __syncwarp();
+          for (int x = 0; i == 0 && x < w.tiles && ok; ++x) {
+            ok = warp_wait(&bars->q_empty[x], (q_phase >> x) & 1, stop);
+            q_phase ^= 1u << x;
+            if (ok && elect_one()) {
+              mbar_arrive_expect_tx(&bars->q_full[x], tile_bytes);
+              // (rows that do not fill the tile leave a gap between its halves)
+              for (int c = 0; c < (a.G * a.tpt == kTile ? 1 : 2); ++c)
+                tma_load_4d(sq + x * kOperand + c * kHalf, &maps.q, 0, w.hk * a.G, w.first + w.tok0 + x * a.tpt, c,
+                            &bars->q_full[x]);
+            }
+            __syncwarp();
+          }
         }
         if (!ok) break;
         if (lane == 0) mbar_arrive(&bars->want);
@@ -716,31 +741,35 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           const int base = (w.t1 - 1 - it) * kTile;
           const int open = max(0, w.low - base), end = min(kTile, w.keys - base);
           uint4* v = reinterpret_cast<uint4*>(ring + vs * kOperand);
+          const int n = 8 * max(0, end - open);  // pieces of one half
+          auto piece = [&](int i) { return i < n ? 8 * open + i : kHalf / 16 + 8 * open + i - n; };
           bool bad = false;
-          for (int half = 0; half < 2; ++half, v += kHalf / 16) {
-            for (int i = 8 * end + lane; i < 8 * kTile; i += 32) v[i] = make_uint4(0, 0, 0, 0);
-            // eight pieces in flight at once; what is found is cleared in a second look
-            for (int i0 = 8 * open + lane; i0 < 8 * end; i0 += 256) {
-              uint4 u[8];
+          // six pieces in flight at once; what is found is cleared in a second look.
+          // (w + w drops the sign and leaves the exponent on top of each half.)
+          for (int i0 = lane; i0 < 2 * n; i0 += 6 * 32) {
+            uint4 u[6];
 #pragma unroll
-              for (int c = 0; c < 8; ++c) u[c] = i0 + 32 * c < 8 * end ? v[i0 + 32 * c] : make_uint4(0, 0, 0, 0);
-              uint32_t any = 0u;
+            for (int c = 0; c < 6; ++c) u[c] = i0 + 32 * c < 2 * n ? v[piece(i0 + 32 * c)] : make_uint4(0, 0, 0, 0);
+            uint32_t m0 = 0u, m1 = 0u;
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                any |= not_finite(u[c].x) | not_finite(u[c].y) | not_finite(u[c].z) | not_finite(u[c].w);
-              if (any == 0u) continue;
-              bad = true;
+            for (int c = 0; c < 6; ++c) {
+              m0 = max_u16x2(max_u16x2(m0, u[c].x + u[c].x), u[c].y + u[c].y);
+              m1 = max_u16x2(max_u16x2(m1, u[c].z + u[c].z), u[c].w + u[c].w);
+            }
+            m0 = max_u16x2(m0, m1);
+            if ((m0 & 0xFFFFu) < 0xFF00u && (m0 >> 16) < 0xFF00u) continue;
+            bad = true;
 #pragma unroll 1
-              for (int i = i0; i < min(8 * end, i0 + 256); i += 32) {
-                uint4 x = v[i];
-                x.x &= ~((not_finite(x.x) >> 15) * 0xFFFFu);
-                x.y &= ~((not_finite(x.y) >> 15) * 0xFFFFu);
-                x.z &= ~((not_finite(x.z) >> 15) * 0xFFFFu);
-                x.w &= ~((not_finite(x.w) >> 15) * 0xFFFFu);
-                v[i] = x;
-              }
+            for (int i = i0; i < min(2 * n, i0 + 6 * 32); i += 32) {
+              uint4 x = v[piece(i)];
+              x.x &= ~((not_finite(x.x) >> 15) * 0xFFFFu);
+              x.y &= ~((not_finite(x.y) >> 15) * 0xFFFFu);
+              x.z &= ~((not_finite(x.z) >> 15) * 0xFFFFu);
+              x.w &= ~((not_finite(x.w) >> 15) * 0xFFFFu);
+              v[piece(i)] = x;
             }
           }
+          for (int i = 8 * end + lane; i < 8 * kTile; i += 32) v[i] = v[kHalf / 16 + i] = make_uint4(0, 0, 0, 0);
           // (kept for the CTA's later items: they then look for such values too)
           if (bad) *const_cast<volatile int*>(&bars->bad) = 1;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -756,20 +785,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       // next is asked for when the last copies of an item are under way, about two
       // key tiles before it ends: asked for sooner, a CTA with a long item would hold
       // back another that an idle one could start (4096 tokens: 174 us for 150).
-      int item = blockIdx.x;
+      int2 item = make_int2(blockIdx.x, blockIdx.y);
       uint32_t asked = 0, wanted = 0;
       Work w;
       while (true) {
         const bool some = load_work(a, item, lane, w);
         if (!some) w.valid = 0;
-        if (some || item < 0) {
+        if (some || item.x < 0) {
           if (!warp_wait(&bars->work_empty[k & 1], ((k >> 1) & 1) ^ 1, stop)) break;
           if (lane == 0) {
             bars->work[k & 1] = w;
             mbar_arrive(&bars->work_full[k & 1]);
           }
           ++k;
-          if (item < 0) break;
+          if (item.x < 0) break;
           if (!warp_wait(&bars->want, wanted++ & 1, stop)) break;
         }
         if (lane == 0) {
@@ -935,11 +964,16 @@ int check_prefill(const exk_prefill* p) {
   return 0;
 }
 
-// Rows [rows, heads, 128] with element strides; box of `tokens` rows of `heads_box` heads, 64 channels.
+// Rows [rows, heads, 128] with element strides as (64 channels, heads, rows, halves):
+// a box of `tokens` rows of `heads_box` heads lands as one or two halves of
+// [tokens][heads_box] 128-byte rows.
 int make_rows_map(CUtensorMap* map, const uint16_t* p, int64_t rows, int heads, int64_t st, int64_t sh, int heads_box,
-                  int tokens) {
-  return make_tmap_3d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, kD, heads, rows, sh * 2, st * 2, 64, heads_box, tokens,
-                      CU_TENSOR_MAP_SWIZZLE_128B);
+                  int tokens, int halves) {
+  const uint64_t dims[4] = {kD / 2, static_cast<uint64_t>(heads), static_cast<uint64_t>(rows), 2};
+  const uint64_t strides[3] = {static_cast<uint64_t>(sh) * 2, static_cast<uint64_t>(st) * 2, kD};
+  const uint32_t box[4] = {kD / 2, static_cast<uint32_t>(heads_box), static_cast<uint32_t>(tokens),
+                           static_cast<uint32_t>(halves)};
+  return make_tmap(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Lets the kernel have its shared memory, once per device (the current one).
@@ -982,16 +1016,18 @@ int launch_prefill(const exk_prefill* p, PrefillArgs& a, const uint16_t* k, int6
   a.ns = p->ns;
   a.scale = p->qk_scale;
   const int64_t slots = prefill_slots(p->N, p->B, a.G);
-  const int64_t grid = slots * p->Hkv * p->ns;
-  if (grid >= (int64_t{1} << 31)) return EXK_EARG;
+  if (slots > 65535) return EXK_EARG;  // over 65,000 blocks of 256 / G tokens
+  const dim3 grid(static_cast<unsigned>(p->Hkv * p->ns), static_cast<unsigned>(slots));
+  a.by_block = (uint64_t{1} << 36) / static_cast<uint64_t>(2 * a.tpt) + 1;
   a.slots = static_cast<int>(slots);
   PrefillMaps maps;
+  const int halves = key_box == kTile ? 2 : 1;  // a page's halves lie apart in the tile
   int r;
-  if ((r = make_rows_map(&maps.q, p->q, p->N, p->Hq, p->q_st, p->q_sh, a.G, a.tpt)) != 0) return r;
-  if ((r = make_rows_map(&maps.k, k, key_rows, p->Hkv, k_st, k_sh, 1, key_box)) != 0) return r;
-  if ((r = make_rows_map(&maps.v, v, key_rows, p->Hkv, v_st, v_sh, 1, key_box)) != 0) return r;
+  if ((r = make_rows_map(&maps.q, p->q, p->N, p->Hq, p->q_st, p->q_sh, a.G, a.tpt, a.G * a.tpt == kTile ? 2 : 1)) != 0) return r;
+  if ((r = make_rows_map(&maps.k, k, key_rows, p->Hkv, k_st, k_sh, 1, key_box, halves)) != 0) return r;
+  if ((r = make_rows_map(&maps.v, v, key_rows, p->Hkv, v_st, v_sh, 1, key_box, halves)) != 0) return r;
   if ((r = allow_smem(device)) != 0) return r;
-  prefill_kernel<<<static_cast<unsigned>(grid), kPrefillThreads, kPrefillSmem, st>>>(a, maps);
+  prefill_kernel<<<grid, kPrefillThreads, kPrefillSmem, st>>>(a, maps);
   if ((r = launch_status()) != 0 || p->ns == 1) return r;
   const int64_t rows = static_cast<int64_t>(p->N) * p->Hq;
   cudaLaunchConfig_t cfg = {};
