@@ -202,11 +202,49 @@ struct Work {
 // x / T for 0 <= x < 2^28, T <= 256, with m = 2^36 / T + 1.
 __device__ __forceinline__ int divide(int x, uint64_t m) { return static_cast<int>((static_cast<uint64_t>(x) * m) >> 36); }
 
-// Block (x, y) of the grid: (KV head, split) and 256-row block, long rows of keys
-// first. Sequence b's blocks take slots cu[b] / T + b, + 1, ... with T = 2 tpt
-// tokens a block: n tokens need at most (n + T - 1) / T, which never reaches
-// sequence b + 1's first slot. False for a slot left over. By a whole warp.
-__device__ __forceinline__ bool load_work(const PrefillArgs& a, int2 block, int lane, Work& w) {
+// The batch as the scheduling warp holds it when it has at most 32 sequences: lane b
+// sequence b's queries and keys, its 256-row blocks, and the blocks of the
+// sequences with more keys (they come first: the calls' last blocks are then short
+// ones). With more sequences nothing of this is used.
+struct Batch {
+  int first, n, L, krow, blocks, before;
+};
+
+// Sequence b's queries and keys; n = 0 where its bounds are not a batch's.
+__device__ __forceinline__ void load_seq(const PrefillArgs& a, int b, Batch& s) {
+  s.first = __ldg(a.cu_q + b);
+  s.n = __ldg(a.cu_q + b + 1) - s.first;
+  if (s.first < 0 || s.n < 0 || s.first > a.N - s.n) s.n = 0;
+  if (a.cu_k != nullptr) {
+    s.krow = __ldg(a.cu_k + b);
+    s.L = __ldg(a.cu_k + b + 1) - s.krow;
+    if (s.krow < 0 || s.L < 0 || s.krow > a.Nk - s.L) s.L = s.krow = 0;
+  } else {
+    s.krow = b * a.k_stride;
+    const int most = a.block_table != nullptr ? a.max_pages * kP : a.k_stride;
+    s.L = max(0, min(__ldg(a.lens + b), most));
+  }
+}
+
+__device__ __forceinline__ Batch load_batch(const PrefillArgs& a, int lane) {
+  Batch s = {0, 0, -1, 0, 0, 0};
+  if (a.B > 32) return s;
+  if (lane < a.B) load_seq(a, lane, s);
+  s.blocks = divide(s.n + 2 * a.tpt - 1, a.by_block);
+#pragma unroll 1
+  for (int b = 0; b < a.B; ++b) {
+    const int L = __shfl_sync(0xFFFFFFFFu, s.L, b), blocks = __shfl_sync(0xFFFFFFFFu, s.blocks, b);
+    if (L > s.L || (L == s.L && b < lane)) s.before += blocks;
+  }
+  return s;
+}
+
+// Block (x, y) of the grid: (KV head, split) and 256-row block of T = 2 tpt tokens,
+// a sequence's blocks with long rows of keys first. With more than 32 sequences,
+// b's blocks take slots cu[b] / T + b, + 1, ...: n tokens need at most (n + T - 1) /
+// T, which never reaches sequence b + 1's first slot, so the map needs no
+// prefix sum. False for a block left over. By a whole warp.
+__device__ __forceinline__ bool load_work(const PrefillArgs& a, const Batch& batch, int2 block, int lane, Work& w) {
   if (block.x < 0) return false;
   const int T = 2 * a.tpt;
   w.split = 0;
@@ -215,30 +253,33 @@ __device__ __forceinline__ bool load_work(const PrefillArgs& a, int2 block, int 
     w.hk = block.x / a.ns;
     w.split = block.x - w.hk * a.ns;
   }
-  const int slot = a.slots - 1 - block.y;
-  int b = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const bool before = b0 + lane < a.B && divide(__ldg(a.cu_q + b0 + lane + 1), a.by_block) + b0 + lane + 1 <= slot;
-    b += __popc(__ballot_sync(0xFFFFFFFFu, before));
-  }
-  if (b >= a.B) return false;
-  w.valid = 1;
-  w.b = b;
-  w.first = __ldg(a.cu_q + b);
-  w.n = __ldg(a.cu_q + b + 1) - w.first;
-  if (w.first < 0 || w.n <= 0 || w.first > a.N - w.n) return false;
-  w.tok0 = (slot - (divide(w.first, a.by_block) + b)) * T;
-  if (w.tok0 < 0 || w.tok0 >= w.n) return false;
-  if (a.cu_k != nullptr) {
-    w.krow = __ldg(a.cu_k + b);
-    w.L = __ldg(a.cu_k + b + 1) - w.krow;
-    if (w.krow < 0 || w.L < 0 || w.krow > a.Nk - w.L) w.L = w.krow = 0;
+  if (a.B <= 32) {
+    const uint32_t mine = __ballot_sync(0xFFFFFFFFu, block.y >= batch.before && block.y < batch.before + batch.blocks);
+    if (mine == 0u) return false;
+    w.b = __ffs(mine) - 1;
+    w.first = __shfl_sync(0xFFFFFFFFu, batch.first, w.b);
+    w.n = __shfl_sync(0xFFFFFFFFu, batch.n, w.b);
+    w.L = __shfl_sync(0xFFFFFFFFu, batch.L, w.b);
+    w.krow = __shfl_sync(0xFFFFFFFFu, batch.krow, w.b);
+    w.tok0 = (__shfl_sync(0xFFFFFFFFu, batch.before + batch.blocks, w.b) - 1 - block.y) * T;
   } else {
-    w.krow = b * a.k_stride;
-    w.L = __ldg(a.lens + b);
-    const int most = a.block_table != nullptr ? a.max_pages * kP : a.k_stride;
-    w.L = max(0, min(w.L, most));
+    const int slot = a.slots - 1 - block.y;
+    w.b = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const bool before = b0 + lane < a.B && divide(__ldg(a.cu_q + b0 + lane + 1), a.by_block) + b0 + lane + 1 <= slot;
+      w.b += __popc(__ballot_sync(0xFFFFFFFFu, before));
+    }
+    if (w.b >= a.B) return false;
+    Batch s;
+    load_seq(a, w.b, s);
+    w.first = s.first;
+    w.n = s.n;
+    w.L = s.L;
+    w.krow = s.krow;
+    w.tok0 = (slot - (divide(w.first, a.by_block) + w.b)) * T;
+    if (w.tok0 < 0 || w.tok0 >= w.n) return false;
   }
+  w.valid = 1;
   w.tiles = w.n - w.tok0 > a.tpt ? 2 : 1;
   w.keys = max(0, w.L - w.n + min(w.tok0 + T, w.n));
   const int all = (w.keys + kTile - 1) / kTile;
@@ -685,11 +726,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
               tma_load_4d(dst, map, 0, w.hk, w.krow + j * kTile, 0, full);
             }
           } else {
-            // one lane per half page; pages past the keys are not loaded (their columns are masked)
-            const int pages = min(kTile / kP, (w.keys - j * kTile + kP - 1) / kP), pg = lane >> 1;
+            // a lane looks each page up; pages past the keys are not loaded (their
+            // columns are masked). One lane issues the copies: issued by sixteen
+            // lanes side by side they are taken one by one all the same, and
+            // slower.
+            const int pages = min(kTile / kP, (w.keys - j * kTile + kP - 1) / kP);
             int row = 0;
-            if (pg < pages) {
-              const int page = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + j * (kTile / kP) + pg);
+            if (lane < pages) {
+              const int page = __ldg(a.block_table + static_cast<int64_t>(w.b) * a.max_pages + j * (kTile / kP) + lane);
               if (page >= 0 && page < a.pool_pages) {
                 row = page * kP;
               } else {
@@ -697,9 +741,17 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
                 row = a.pool_pages * kP;  // outside the map: zeros
               }
             }
-            if (lane == 0) mbar_arrive_expect_tx(full, pages * (2 * 64 * 2 * kP));
+            const int hk = __shfl_sync(0xFFFFFFFFu, w.hk, 0), n = __shfl_sync(0xFFFFFFFFu, pages, 0);
+            if (elect_one()) mbar_arrive_expect_tx(full, n * (2 * 64 * 2 * kP));
             __syncwarp();
-            if (pg < pages) tma_load_4d(dst + (lane & 1) * kHalf + pg * (kP * 128), map, 0, w.hk, row, lane & 1, full);
+#pragma unroll
+            for (int pg = 0; pg < kTile / kP; ++pg) {
+              const int at = __shfl_sync(0xFFFFFFFFu, row, pg);
+              if (pg < n && elect_one()) {
+                tma_load_4d(dst + pg * (kP * 128), map, 0, hk, at, 0, full);
+                tma_load_4d(dst + kHalf + pg * (kP * 128), map, 0, hk, at, 1, full);
+              }
+            }
           }
           __syncwarp();
           for (int x = 0; i == 0 && x < w.tiles && ok; ++x) {
@@ -785,11 +837,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       // next is asked for when the last copies of an item are under way, about two
       // key tiles before it ends: asked for sooner, a CTA with a long item would hold
       // back another that an idle one could start (4096 tokens: 174 us for 150).
+      const Batch batch = load_batch(a, lane);
       int2 item = make_int2(blockIdx.x, blockIdx.y);
       uint32_t asked = 0, wanted = 0;
       Work w;
       while (true) {
-        const bool some = load_work(a, item, lane, w);
+        const bool some = load_work(a, batch, item, lane, w);
         if (!some) w.valid = 0;
         if (some || item.x < 0) {
           if (!warp_wait(&bars->work_empty[k & 1], ((k >> 1) & 1) ^ 1, stop)) break;
@@ -1058,8 +1111,14 @@ extern "C" int exk_prefill_splits(int N, int B, int Hq, int Hkv, int64_t max_key
   if (Hq / Hkv > 16) return EXK_EHEADS;
   const int64_t items = prefill_slots(N, B, Hq / Hkv) * Hkv;
   const int64_t tiles = (max_keys + kTile - 1) / kTile;
-  // whole waves of CTAs need no splits; else as many as fill the SMs once, of four key tiles at least
-  const int64_t fit = items > 0 ? num_sms / items : 1;
+  if (items == 0) return 1;
+  // As many as fill the SMs once; where the partials are few (16 MB: under 3 us), and
+  // the lengths of several sequences may differ, twice. Four key tiles to a
+  // split at least. (16 sequences of 2 to 8 tokens over 1,000 to 4,000 keys:
+  // 109 us, unsplit 115 us.)
+  int64_t fit = num_sms / items;
+  const int64_t twice = (2 * static_cast<int64_t>(num_sms) + items - 1) / items;
+  if (B > 1 && twice * N * Hq * (kD + 2) * 4 <= (int64_t{16} << 20)) fit = twice;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({fit, tiles / 4, kMaxSplits})));
 }
 
