@@ -206,7 +206,7 @@ __device__ __forceinline__ void token_rows(const Append& a, int64_t work, int st
   const int b = t.cu_seqlens == nullptr ? tok : find_seq(t.cu_seqlens, t.B, 1, 0, tok, lane);
   if (b >= t.B) return;  // behind the last sequence
   const Seq s = load_seq(t, b);
-  if (s.n <= 0) return;
+  if (tok < s.first || tok - s.first >= s.n) return;  // (rows before the first sequence)
   const int pos = s.start + tok - s.first;
   const bool ok = position_ok(t, pos);
   Turn<4> turn;

@@ -221,8 +221,9 @@ __device__ __forceinline__ void load_seq(const PrefillArgs& a, int b, Batch& s) 
     if (s.krow < 0 || s.L < 0 || s.krow > a.Nk - s.L) s.L = s.krow = 0;
   } else {
     s.krow = b * a.k_stride;
-    const int most = a.block_table != nullptr ? a.max_pages * kP : a.k_stride;
-    s.L = max(0, min(__ldg(a.lens + b), most));
+    const int most = a.block_table != nullptr ? a.max_pages * kP : a.k_stride, L = __ldg(a.lens + b);
+    if (L > most) set_status(a.status, EXK_S_POSITION);  // keys past the table or the workspace are not seen
+    s.L = max(0, min(L, most));
   }
 }
 

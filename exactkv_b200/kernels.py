@@ -602,8 +602,8 @@ def _coded_pool(c, dev, write):
         B, sm, cap, cnt = c.B, c.sm, getattr(c, "cap", None), getattr(c, "cnt", None)
     if sm.device != dev:
         raise ValueError("the pools must be on q's device")
-    if write and (cap is None or cnt is None):
-        raise ValueError("a pool that is written needs its raw pool's capacity (cap) and counter (cnt)")
+    if write and (cap is None or cnt is None or cnt.dtype is not torch.int32 or cnt.device != dev):
+        raise ValueError("a pool that is written needs its raw pool's capacity (cap) and int32 counter (cnt)")
     return view, H, B * TS // P, cap, cnt
 
 
@@ -696,7 +696,9 @@ def attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None):
     Nk, Hkv = k.shape[:2]
     k_at, k_st, k_sh = _rows(k, "k", Nk, Hkv, q.device)
     v_at, v_st, v_sh = _rows(v, "v", Nk, Hkv, q.device)
-    a, out, N, B, ws = _prefill_args(q, cu_seqlens, Hkv, Nk, out)
+    # (the plan only: the lengths are on the device, a sequence has about Nk / B keys)
+    many = max(1, cu_seqlens.numel() - 1)
+    a, out, N, B, ws = _prefill_args(q, cu_seqlens, Hkv, Nk if many == 1 else min(Nk, 2 * Nk // many), out)
     if cu_seqlens_k is None:
         if Nk != N:
             raise ValueError("k and v rows differ from q's: give cu_seqlens_k")
@@ -734,7 +736,8 @@ def attention_prefill_paged(q, kc, vc, block_table, seq_lens, cu_seqlens, max_le
     attention_paged takes them): the queries are the last tokens of sequences of
     seq_lens[b] tokens whose pages block_table names, as rope_append_paged left
     them. max_len (host, at least every seq_lens[b]; default max_pages * 16)
-    bounds the workspace of B * max_len decoded rows. Bit-identical to
+    bounds the workspace of B * max_len decoded rows; a longer sequence is cut
+    and reported by check_status(). Bit-identical to
     attention_prefill_reference_paged for the same values and max_len."""
     kv, H, pages, _, _ = _coded_pool(kc, q.device, False)
     vv, vH, v_pages, _, _ = _coded_pool(vc, q.device, False)

@@ -60,7 +60,7 @@ extern "C" {
 #define EXK_S_DRAIN_TIMEOUT  5  /* in-flight TMA copies did not land within 2 s */
 #define EXK_S_PEER_TIMEOUT   6  /* a peer merge waited > 2 s for another GPU's signal */
 #define EXK_S_PAGE_INDEX     7  /* a block-table entry named a page outside the pool */
-#define EXK_S_POSITION       8  /* a token's position or tail slot was out of range (not stored) */
+#define EXK_S_POSITION       8  /* a token's position or tail slot, or a length, was out of range */
 
 /* One compressed cache (keys or values of one layer): the six buffers of the
  * format above. raw_rows is the number of rows `raw` holds; indices at or
@@ -367,7 +367,8 @@ int exk_rope_append_compressed(const exk_append *a, const exk_cview *k, int64_t 
  * sequence b's at rows [cu_q[b], cu_q[b+1]) (int32, device), its last query at
  * its last key: query i of n sees keys j <= i + L - n of L. A query that sees
  * no key gives zeros; rows at and past cu_q[B] of `out` (strides o_st, o_sh)
- * are left alone. Hq = G * Hkv, G <= 16. ns splits of each row's keys
+ * are left alone. Hq = G * Hkv, G <= 16; at most 65,535 blocks of 2 *
+ * floor(128 / G) tokens, N / block + B of them (EXK_EARG). ns splits of each row's keys
  * (exk_prefill_splits): with ns > 1 po [N * Hq, ns, 128], pm, pl [N * Hq, ns]
  * fp32 hold their partials. qk_scale: log2(e) / sqrt(128). */
 typedef struct exk_prefill {
@@ -395,14 +396,16 @@ int exk_attention_prefill(const exk_prefill *a, const uint16_t *k, int64_t k_st,
 /* Keys and values in bf16 pools [pool_pages * 16, Hkv, 128]: sequence b's
  * first seq_lens[b] tokens (its queries' own among them) in the pages that
  * row b of block_table [B, max_pages] names. An entry outside the pool reads
- * as zeros (EXK_S_PAGE_INDEX). */
+ * as zeros (EXK_S_PAGE_INDEX); a length past the table is cut to it
+ * (EXK_S_POSITION). */
 int exk_attention_prefill_paged(const exk_prefill *a, const uint16_t *k, const uint16_t *v, int pool_pages,
                                 const int32_t *block_table, int max_pages, const int32_t *seq_lens,
                                 int32_t *status, int device, void *stream);
 
 /* The same over compressed pools; bit-identical for the same values. k_rows
  * and v_rows are workspaces of [B * max_len, Hkv, 128] bf16, max_len (a
- * multiple of 16) at least every seq_lens[b]; keys past max_len are not seen. */
+ * multiple of 16) at least every seq_lens[b] (a longer sequence is cut to its
+ * first max_len keys: EXK_S_POSITION). */
 int exk_attention_prefill_paged_compressed(const exk_prefill *a, const exk_cview *k, const exk_cview *v,
                                            int pool_pages, const int32_t *block_table, int max_pages,
                                            const int32_t *seq_lens, uint16_t *k_rows, uint16_t *v_rows,

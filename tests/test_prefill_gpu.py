@@ -198,7 +198,8 @@ def test_paged_equals_contiguous_bit_for_bit(lens, klens, Hq, Hkv):
     wide_b = ekv.attention_prefill_reference_paged(q, kb, vb, table, sl, cu)
     assert same_bits(wide_b, ekv.attention_prefill_paged(q, kc, vc, table, sl, cu))
     check(wide_b, q, k, v, lens, klens)
-    if sum(klens) <= 2048:                       # no split on either side: the same order of sums
+    plan = lambda keys: kernels.lib.exk_prefill_splits(sum(lens), len(lens), Hq, Hkv, keys, kernels.num_sms())  # noqa: E731
+    if plan(-(-most // 16) * 16) == plan(sum(klens)) == 1:       # split on neither side: the same order of sums
         assert same_bits(o_b, ekv.attention_prefill(q, k, v, cu, ck))
     kernels.check_status()
 
@@ -219,6 +220,70 @@ def test_pages_outside_the_pool_read_as_zeros_and_are_reported():
         with pytest.raises(RuntimeError, match="outside the pool"):
             kernels.check_status()
         check(out, q, k0, v0, [20], [300])
+
+
+@pytest.mark.gpu
+def test_lengths_past_the_table_or_the_workspace_are_cut_and_reported():
+    q, _, _ = inputs(5, 1, 8, 2, seed=33)
+    k, v, kb, vb, kc, vc, table, sl = _pools([100, 64], 2, seed=34, max_extra=0)
+    cu = offsets([3, 2]).cuda()
+    long = torch.tensor([500, 64], dtype=torch.int32, device="cuda")
+    for call, a, b, lens, kw in ((ekv.attention_prefill_reference_paged, kb, vb, long, {}),
+                                 (ekv.attention_prefill_paged, kc, vc, long, {}),
+                                 (ekv.attention_prefill_paged, kc, vc, sl, dict(max_len=64))):
+        out = call(q, a, b, table, lens, cu, **kw)
+        with pytest.raises(RuntimeError, match="length"):
+            kernels.check_status()
+        check(out[3:], q[3:], k[100:], v[100:], [2], [64])         # the other sequence is as it should be
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pad", [0, 3])
+def test_many_sequences(pad):
+    """More sequences than a warp holds (the other way to map blocks), some empty,
+    with rows before the first and after the last that belong to none."""
+    lens = [(7 * i) % 41 for i in range(70)]
+    klens = [n + (13 * i) % 150 for i, n in enumerate(lens)]
+    Hq, Hkv, n = 8, 2, sum(lens)
+    q, _, _ = inputs(n + 2 * pad, 1, Hq, Hkv, seed=90)
+    _, k, v = inputs(1, sum(klens), Hq, Hkv, seed=91)
+    hold = torch.full_like(q, 5.0)
+    out = ekv.attention_prefill(q, k, v, offsets(lens).cuda() + pad, offsets(klens).cuda(), out=hold)
+    check(out[pad:], q[pad:pad + n], k, v, lens, klens)
+    assert (hold[:pad] == 5).all() and (hold[pad + n:] == 5).all()
+    # a sequence by itself, where the plan may split its keys otherwise
+    a = b = pad
+    for i, (m, L) in enumerate(zip(lens, klens)):
+        if m and L and i % 9 == 0:
+            kk, vv = k[b - pad:b - pad + L], v[b - pad:b - pad + L]
+            one = ekv.attention_prefill(q[a:a + m], kk, vv, offsets([m]).cuda(), offsets([L]).cuda())
+            check(one, q[a:a + m], kk, vv, [m], [L])
+        a, b = a + m, b + L
+    kernels.check_status()
+
+
+@pytest.mark.gpu
+def test_pools_past_32_bit_offsets():
+    """Pools of 2.7e9 values: the pages in use lie at their end."""
+    Hq, Hkv, pages = 16, 8, 165_000
+    lens = [300, 70]
+    k = synthetic.make_kv(1, sum(lens), Hkv, seed=95, key=True)[0]
+    v = synthetic.make_kv(1, sum(lens), Hkv, seed=96, key=False)[0]
+    q, _, _ = inputs(sum(lens), 1, Hq, Hkv, seed=97)
+    table = torch.full((2, 19), -1, dtype=torch.int32)
+    table[0] = pages - 1 - torch.arange(19)
+    table[1, :5] = pages - 40 + torch.arange(5)
+    table, sl, cu = table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), offsets(lens).cuda()
+    ident = torch.cat([torch.ones(400, 64), torch.zeros(400, 64)], 1).cuda()
+    kb, vb = (torch.zeros(1, pages * 16, Hkv, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ekv.rope_append_reference_paged(q, k, v, ident, kb, vb, table, sl, cu)
+    o = ekv.attention_prefill_reference_paged(q, kb, vb, table, sl, cu)
+    check(o, q, k, v, lens, lens)
+    del kb, vb
+    kc, vc = (ekv.PagedCompressedKV(pages, Hkv, D, 2, reserve=0.001) for _ in range(2))
+    ekv.rope_append_paged(q, k, v, ident, kc, vc, table, sl, cu)
+    assert same_bits(ekv.attention_prefill_paged(q, kc, vc, table, sl, cu), o)
+    kernels.check_status()
 
 
 @pytest.mark.gpu

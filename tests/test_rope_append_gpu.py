@@ -195,6 +195,29 @@ def test_raw_slots_follow_sequence_page_head_order():
 
 
 @pytest.mark.gpu
+def test_many_sequences_and_rows_before_the_first():
+    """70 sequences, some without new tokens, in a batch whose first rows belong to
+    none: those rows and their queries are left alone."""
+    B, Hq, Hkv, pad = 70, 4, 2, 5
+    new = [(5 * i) % 23 for i in range(B)]
+    q, k, v = tokens(sum(new) + pad, Hq, Hkv, seed=80)
+    m = Model(B, Hkv, 3, seed=14)
+    cu, sl = offsets(new) + pad, ints(new)
+    out = [torch.full_like(q, 5.0) for _ in range(2)]
+    ekv.rope_append_reference_paged(q, k, v, m.cs, m.kb, m.vb, m.table, sl, cu, q_out=out[0])
+    ekv.rope_append_paged(q, k, v, m.cs, m.kc, m.vc, m.table, sl, cu, q_out=out[1])
+    kernels.check_status()
+    assert same_bits(*out) and (out[0][:pad] == 5).all()
+    at = pad
+    for b, n in enumerate(new):
+        assert same_bits(out[0][at:at + n].cpu(), rotated(q[at:at + n], m.cs[:n]))
+        m.k[b], m.v[b] = rotated(k[at:at + n], m.cs[:n]), v[at:at + n].cpu()
+        m._count(b, 0, n)
+        at += n
+    m.check()
+
+
+@pytest.mark.gpu
 def test_norm_before_the_rotation():
     Hq, Hkv, new, start = 12, 4, [40, 1, 3], [3, 15, 0]
     g = torch.Generator(device="cuda").manual_seed(1)
