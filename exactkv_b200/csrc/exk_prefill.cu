@@ -950,53 +950,70 @@ struct Unpack {
   int B, Hkv, max_pages, pool_pages, pages;  // pages: k_stride / 16
 };
 
+// Eight lanes to a row, 8 bytes of sm's halves and of code to a lane; all rows
+// of the page are loaded before the first is decoded.
 __global__ void __launch_bounds__(256) unpack_kernel(const __grid_constant__ Unpack u) {
-  allow_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t ph = static_cast<int64_t>(blockIdx.x) * 8 + warp;
   const int h = static_cast<int>(ph % u.Hkv);
   const int pg = static_cast<int>((ph / u.Hkv) % u.pages);
   const int64_t b = ph / (static_cast<int64_t>(u.Hkv) * u.pages);
   if (b >= u.B) return;
-  const int L = min(__ldg(u.lens + b), static_cast<int>(u.k_stride));
-  if (pg * kP >= L) return;
+  const int L = min(__ldg(u.lens + b), static_cast<int>(u.k_stride)) - pg * kP;  // rows of the page that are wanted
+  if (L <= 0) return;
   const int pool = __ldg(u.block_table + b * u.max_pages + pg);
-  const exk_cview& c = u.c[blockIdx.y];
-  const int q = lane & 15, th = lane >> 4;
-  uint16_t* out = u.out[blockIdx.y] + ((b * u.k_stride + static_cast<int64_t>(pg) * kP + 8 * th) * u.Hkv + h) * kD;
-  const bool bad = pool < 0 || pool >= u.pool_pages;
-  if (bad) set_status(u.status, EXK_S_PAGE_INDEX);
-  const int64_t page = bad ? 0 : static_cast<int64_t>(pool) * u.Hkv + h;
-  const uint32_t rm = bad ? 0u : static_cast<uint32_t>(c.rowmask[page]) & 0xFFFFu;
-  const int32_t ro = bad ? 0 : c.rowoff[page];
-  const uint32_t bl = *reinterpret_cast<const uint32_t*>(c.base + page * kD + 4 * q);
-  const uint32_t bh = *reinterpret_cast<const uint32_t*>(c.base + page * kD + 64 + 4 * q);
+  const exk_cview& v = u.c[blockIdx.y];
+  const int c = lane & 7, r4 = lane >> 3;
+  uint16_t* out = u.out[blockIdx.y] + ((b * u.k_stride + static_cast<int64_t>(pg) * kP + r4) * u.Hkv + h) * kD + 8 * c;
+  const int64_t step = static_cast<int64_t>(4) * u.Hkv * kD;
+  if (pool < 0 || pool >= u.pool_pages) {
+    set_status(u.status, EXK_S_PAGE_INDEX);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int tok = th * 8 + i;
-    uint32_t w0 = 0u, w1 = 0u, w2 = 0u, w3 = 0u;
-    if (pg * kP + tok >= L) break;
-    if (bad) {
-    } else if ((rm >> tok) & 1u) {
-      const int64_t ridx = static_cast<int64_t>(ro) + __popc(rm & ((1u << tok) - 1u));
-      if (ridx < 0 || ridx >= c.raw_rows) {
-        set_status(u.status, EXK_S_RAW_INDEX);
+    for (int s = 0; s < 4; ++s)
+      if (4 * s + r4 < L) {
+        uint4* o = reinterpret_cast<uint4*>(out + s * step);
+        o[0] = o[8] = make_uint4(0, 0, 0, 0);
+      }
+    return;
+  }
+  const int64_t page = static_cast<int64_t>(pool) * u.Hkv + h;
+  const int64_t token = (static_cast<int64_t>(pool) * kP + r4) * u.Hkv + h;
+  const uint32_t rm = static_cast<uint32_t>(__ldg(v.rowmask + page)) & 0xFFFFu;
+  const int32_t ro = __ldg(v.rowoff + page);
+  const uint2 bl = __ldg(reinterpret_cast<const uint2*>(v.base + page * kD + 8 * c));
+  const uint2 bh = __ldg(reinterpret_cast<const uint2*>(v.base + page * kD + 64 + 8 * c));
+  uint2 sl[4], sh[4], cw[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int64_t at = token + static_cast<int64_t>(4) * s * u.Hkv;
+    sl[s] = __ldg(reinterpret_cast<const uint2*>(v.sm + at * kD + 8 * c));
+    sh[s] = __ldg(reinterpret_cast<const uint2*>(v.sm + at * kD + 64 + 8 * c));
+    cw[s] = __ldg(reinterpret_cast<const uint2*>(v.code + at * (kD / 2) + 8 * c));
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int row = 4 * s + r4;
+    if (row >= L) break;
+    uint4 lo, hi;
+    if ((rm >> row) & 1u) {
+      const int64_t ridx = static_cast<int64_t>(ro) + __popc(rm & ((1u << row) - 1u));
+      lo = hi = make_uint4(0, 0, 0, 0);
+      if (ridx >= 0 && ridx < v.raw_rows) {
+        const uint4* p = reinterpret_cast<const uint4*>(v.raw + ridx * kD + 8 * c);
+        lo = __ldg(p);
+        hi = __ldg(p + 8);
       } else {
-        const uint16_t* r = c.raw + ridx * kD;
-        const uint2 lo = *reinterpret_cast<const uint2*>(r + 4 * q), hi = *reinterpret_cast<const uint2*>(r + 64 + 4 * q);
-        w0 = lo.x; w1 = lo.y; w2 = hi.x; w3 = hi.y;
+        set_status(u.status, EXK_S_RAW_INDEX);
       }
     } else {
-      const int64_t row = (static_cast<int64_t>(pool) * kP + tok) * u.Hkv + h;
-      const uint32_t sl = *reinterpret_cast<const uint32_t*>(c.sm + row * kD + 4 * q);
-      const uint32_t sh = *reinterpret_cast<const uint32_t*>(c.sm + row * kD + 64 + 4 * q);
-      const uint32_t cw = *reinterpret_cast<const uint32_t*>(c.code + row * (kD / 2) + 4 * q);
-      dec4(sl, lo_nibbles(cw), bl & 0x7F7F7F7Fu, bl, w0, w1);
-      dec4(sh, hi_nibbles(cw), bh & 0x7F7F7F7Fu, bh, w2, w3);
+      dec4(sl[s].x, lo_nibbles(cw[s].x), bl.x & 0x7F7F7F7Fu, bl.x, lo.x, lo.y);
+      dec4(sl[s].y, lo_nibbles(cw[s].y), bl.y & 0x7F7F7F7Fu, bl.y, lo.z, lo.w);
+      dec4(sh[s].x, hi_nibbles(cw[s].x), bh.x & 0x7F7F7F7Fu, bh.x, hi.x, hi.y);
+      dec4(sh[s].y, hi_nibbles(cw[s].y), bh.y & 0x7F7F7F7Fu, bh.y, hi.z, hi.w);
     }
-    uint16_t* o = out + static_cast<int64_t>(i) * u.Hkv * kD;
-    *reinterpret_cast<uint2*>(o + 4 * q) = make_uint2(w0, w1);
-    *reinterpret_cast<uint2*>(o + 64 + 4 * q) = make_uint2(w2, w3);
+    uint4* o = reinterpret_cast<uint4*>(out + s * step);
+    o[0] = lo;
+    o[8] = hi;
   }
 }
 
@@ -1112,15 +1129,40 @@ extern "C" int exk_prefill_splits(int N, int B, int Hq, int Hkv, int64_t max_key
   if (Hq / Hkv > 16) return EXK_EHEADS;
   const int64_t items = prefill_slots(N, B, Hq / Hkv) * Hkv;
   const int64_t tiles = (max_keys + kTile - 1) / kTile;
-  if (items == 0) return 1;
-  // As many as fill the SMs once; where the partials are few (16 MB: under 3 us), and
-  // the lengths of several sequences may differ, twice. Four key tiles to a
-  // split at least. (16 sequences of 2 to 8 tokens over 1,000 to 4,000 keys:
-  // 109 us, unsplit 115 us.)
-  int64_t fit = num_sms / items;
-  const int64_t twice = (2 * static_cast<int64_t>(num_sms) + items - 1) / items;
-  if (B > 1 && twice * N * Hq * (kD + 2) * 4 <= (int64_t{16} << 20)) fit = twice;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({fit, tiles / 4, kMaxSplits})));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(tiles / 4, kMaxSplits));  // four key tiles to a split at least
+  if (items == 0 || items >= 4 * static_cast<int64_t>(num_sms)) return 1;
+  const double row_bytes = static_cast<double>(N) * Hq * (kD + 2) * 4;  // of one split's partials
+  if (B > 1) {
+    // As many as fill the SMs once; where the partials are few (16 MB: under 3 us)
+    // twice, since the lengths may differ: 16 sequences of 2 to 8 tokens over
+    // 1,000 to 4,000 keys 109 us, unsplit 115 us. (Splits for the longest
+    // sequences alone, cut to an SM's share on the device, measured slower: 4
+    // sequences of 168 to 484 tokens over 2,600 to 7,500 keys 153 us for 141.)
+    int64_t ns = num_sms / items;
+    const int64_t twice = (2 * static_cast<int64_t>(num_sms) + items - 1) / items;
+    if (twice * row_bytes <= 16e6) ns = twice;
+    return static_cast<int>(std::max<int64_t>(1, std::min(ns, most)));
+  }
+  // One sequence: its blocks see max_keys - N keys of context and up to N more. The
+  // estimate counts waves of blocks (1.8 us a key tile, 4 us a block) where the
+  // context outweighs the blocks' differences, else the longest block or an SM's
+  // share, and the partials' traffic. (2,048 tokens over 32,768 keys, 28 heads to 4:
+  // 228 blocks, three splits 848 us, unsplit 900 us.)
+  const double context = static_cast<double>(std::max<int64_t>(0, max_keys - N));
+  double best = 0.;
+  int64_t choice = 1;
+  for (int64_t ns = 1; ns <= most; ++ns) {
+    const double longest = 1.8 * static_cast<double>((tiles + ns - 1) / ns) + 4.;
+    const double waves = static_cast<double>((items * ns + num_sms - 1) / num_sms);
+    const double share = static_cast<double>(items) * (1.8 * (context + 0.5 * N) / kTile + 4. * ns) / num_sms;
+    double us = context > N ? waves * longest : std::max(longest, share);
+    if (ns > 1) us += 4. + 2. * row_bytes * ns / 6.5e6;
+    if (ns == 1 || us < best) {
+      best = us;
+      choice = ns;
+    }
+  }
+  return static_cast<int>(choice);
 }
 
 extern "C" int exk_attention_prefill(const exk_prefill* p, const uint16_t* k, int64_t k_st, int64_t k_sh,

@@ -153,9 +153,12 @@ def test_values_and_keys_that_are_not_finite_reach_only_the_rows_that_see_them(l
     k2[at, 0, 5] = bad
     out = ekv.attention_prefill(q, k2, v, cu, ck)
     assert same_bits(out[~sees], clean[~sees]) and same_bits(out[:, 4:], clean[:, 4:])
-    # garbage rows of a larger buffer behind the last key
-    pad = lambda t: torch.cat([t, torch.full((200, Hkv, D), bad, dtype=torch.bfloat16, device="cuda")])  # noqa: E731
-    assert same_bits(ekv.attention_prefill(q, pad(k), pad(v), cu, ck), clean)
+    # rows of a larger buffer behind the last key: whatever they hold, the same bits
+    # (the plan of the splits goes by the buffer's size, so both calls have one)
+    pad = lambda t, x: torch.cat([t, torch.full((200, Hkv, D), x, dtype=torch.bfloat16, device="cuda")])  # noqa: E731
+    want = ekv.attention_prefill(q, pad(k, 1.0), pad(v, 1.0), cu, ck)
+    assert same_bits(ekv.attention_prefill(q, pad(k, bad), pad(v, bad), cu, ck), want)
+    check(want, q, k, v, lens, klens)
 
 
 def _pools(lens, Hkv, seed, spare=5, max_extra=2):
