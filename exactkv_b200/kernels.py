@@ -538,7 +538,7 @@ def _heads(q, Hkv):
 def _new_rows(out, name, q, N, Hq):
     """The output for q's rows: `out`, checked, or a new tensor, with its address and strides."""
     if out is None:
-        out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         return out, (out.data_ptr(), Hq * D, D)
     return out, _rows(out, name, N, Hq, q.device)
 
@@ -669,9 +669,11 @@ def _prefill_args(q, cu_seqlens, Hkv, max_keys, out):
         raise ValueError("cu_seqlens must hold B + 1 offsets")
     cu = _index(cu_seqlens, "cu_seqlens", (B + 1,), dev)
     out, (o_at, o_st, o_sh) = _new_rows(out, "out", q, N, Hq)
-    ns = lib.exk_prefill_splits(N, B, Hq, Hkv, max_keys, num_sms(dev.index))
-    if ns < 0:
-        check(ns, "exk_prefill_splits")
+    ns = 1
+    if max_keys > 896:                      # (a split has at least four tiles of 128 keys)
+        ns = lib.exk_prefill_splits(N, B, Hq, Hkv, max_keys, num_sms(dev.index))
+        if ns < 0:
+            check(ns, "exk_prefill_splits")
     ws, o, m, l = None, 0, 0, 0
     if ns > 1:
         rows = N * Hq * ns
