@@ -594,7 +594,7 @@ extern "C" int exk_rope_append_bf16(const exk_append* t, uint16_t* k_pool, uint1
                                     void* stream) {
   int r = check_append(t);
   if (r != 0) return r;
-  if (k_pool == nullptr || v_pool == nullptr) return EXK_EARG;
+  if (k_pool == nullptr || v_pool == nullptr || k_pool == v_pool) return EXK_EARG;
   if (!aligned16(k_pool) || !aligned16(v_pool)) return EXK_EALIGN;
   if (t->N == 0) return 0;
   DeviceScope scope;
@@ -625,6 +625,7 @@ extern "C" int exk_rope_append_compressed(const exk_append* t, const exk_cview* 
   int r = check_append(t);
   if (r != 0) return r;
   if (k == nullptr || v == nullptr || k_cnt == nullptr || v_cnt == nullptr || scratch == nullptr) return EXK_EARG;
+  if (k->sm == v->sm || k->raw == v->raw || k_cnt == v_cnt) return EXK_EARG;  // keys and values have pools of their own
   const exk_cview* c[2] = {k, v};
   const int64_t cap[2] = {k_cap, v_cap};
   int32_t* cnt[2] = {k_cnt, v_cnt};

@@ -456,22 +456,23 @@ def test_entry_points_refuse_before_any_launch():
     def app(**kw):
         return APPEND.pack(*{**fits, **{n: v or 0 for n, v in kw.items()}}.values())
 
-    bf = lambda a, k=at: lib.exk_rope_append_bf16(a, k, at, None, 0, None)  # noqa: E731
+    bf = lambda a, k=at: lib.exk_rope_append_bf16(a, k, 2 * at, None, 0, None)  # noqa: E731
     assert lib.exk_rope_append_bf16(None, at, at, None, 0, None) == -1
     for kw in (dict(q=None), dict(B=0), dict(Hq=7), dict(N=5), dict(q_norm=at), dict(max_pages=0), dict(pool_pages=0),
                dict(seq_lens=None), dict(rope_rows=0), dict(N=-1)):
         assert bf(app(**kw)) == -1, kw
-    assert bf(app(q_st=1028)) == -2 and bf(app(k=at + 8)) == -2 and bf(app(), at + 2) == -2 and bf(app(), None) == -1
+    assert bf(app(q_st=1028)) == -2 and bf(app(k=at + 8)) == -2 and bf(app(), at + 2) == -2 and bf(app(), None) == -1 and bf(app(), 2 * at) == -1
     n = lib.exk_rope_append_scratch(4, 4, 2, 0)
-    cv = CView(at, at, at, at, at, at, 1000 + 4 * 2 * 16)
+    cv, other = (CView(x, x, x, x, x, x, 1000 + 4 * 2 * 16) for x in (at, 2 * at))
     short = CView(at, at, at, at, at, at, 1000 + 3 * 2 * 16)
 
-    def coded(a=None, k=cv, cap=1000, scratch=at, bytes_=n):
-        return lib.exk_rope_append_compressed(a or app(), ctypes.byref(k), cap, at, ctypes.byref(cv), 1000, at, scratch,
-                                              bytes_, None, 0, None)
+    def coded(a=None, k=cv, cap=1000, scratch=at, bytes_=n, cnt=at):
+        return lib.exk_rope_append_compressed(a or app(), ctypes.byref(k), cap, cnt, ctypes.byref(other), 1000, 2 * at,
+                                              scratch, bytes_, None, 0, None)
 
     assert coded(bytes_=n - 1) == -1 and coded(k=short) == -1 and coded(cap=-1) == -1 and coded(scratch=None) == -1
     assert coded(scratch=at + 4) == -2 and coded(a=app(Hq=7)) == -1
+    assert coded(k=other) == -1 and coded(cnt=2 * at) == -1      # one pool, or one counter, for keys and values
 
     pnames = "q out q_st q_sh o_st o_sh cu_q po pm pl N B Hq Hkv ns qk_scale".split()
     pfits = dict(zip(pnames, (at, at, 1024, 128, 1024, 128, at, 0, 0, 0, 4, 1, 8, 2, 1, 0.1)))
