@@ -13,8 +13,8 @@
 //
 // Long calls are bound by memory: 11,016 tokens of 32 + 8 + 8 heads into bf16 pages
 // take 44.4 us (276 MB, 6.2 TB/s; with the norm 49 us), 9,529 of 28 + 4 + 4 into
-// coded pages 44 us (22 the queries, 14 the encoding, 9 placing the raw rows); a
-// step of 64 sequences 2.7 us, of 32 into coded pages 8.9 us.
+// coded pages 36 us (14 the encoding, 22 the queries, the raw rows' places beside
+// them); a step of 64 sequences 3 us, of 32 into coded pages 9 us.
 #include <algorithm>
 
 #include "exk_device.cuh"
@@ -411,15 +411,10 @@ __device__ __forceinline__ void write_open(const Append& a, const Item& it, int 
   }
 }
 
-// Blocks below `enc_blocks`: the items; the others rotate the queries.
 template <bool NORM>
-__global__ void __launch_bounds__(kRowWarps * 32) append_encode_kernel(const __grid_constant__ Append a, int enc_blocks, int steps) {
+__global__ void __launch_bounds__(kRowWarps * 32) append_encode_kernel(const __grid_constant__ Append a) {
   allow_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (static_cast<int>(blockIdx.x) >= enc_blocks) {
-    token_rows<false, NORM>(a, static_cast<int64_t>(blockIdx.x - enc_blocks) * kRowWarps + warp, steps, lane);
-    return;
-  }
   if (blockIdx.x == 0 && threadIdx.x < 2) a.base_cnt[threadIdx.x] = *a.cnt[threadIdx.x];
   const int work = blockIdx.x * kRowWarps + warp;
   if (work >= 2 * a.items) return;
@@ -466,17 +461,25 @@ __global__ void __launch_bounds__(kRowWarps * 32) append_encode_kernel(const __g
 constexpr int kPlaceItems = 64;     // items of one CTA of append_place_kernel
 constexpr int kPlaceThreads = 256;  // eight warps, eight items each
 
-// blockIdx.y: keys, values. The CTA adds up the counts of all items before its
-// own (bytes: 65,536 items are 16 loads of 16 bytes per thread), scans its own,
-// writes the offsets and copies the escaped rows.
+// Blocks below 2 * chunks place a chunk of items, keys and values in turn: the CTA
+// adds up the counts of all items before its own (bytes: 65,536 items are 16 loads
+// of 16 bytes per thread), scans its own, writes the offsets and copies the
+// escaped rows. That is a chain of look-ups with little to move, so the other
+// blocks rotate the queries beside it, and start without waiting for the first
+// kernel (9,529 tokens: 36 us; rotated in the first kernel 44 us).
 template <bool NORM>
-__global__ void __launch_bounds__(kPlaceThreads) append_place_kernel(const __grid_constant__ Append a) {
+__global__ void __launch_bounds__(kPlaceThreads) append_place_kernel(const __grid_constant__ Append a, int chunks, int steps) {
   __shared__ int s_before[kPlaceThreads / 32];
   __shared__ int s_count[kPlaceItems], s_off[kPlaceItems];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (static_cast<int>(blockIdx.x) >= 2 * chunks) {
+    token_rows<false, NORM>(a, static_cast<int64_t>(blockIdx.x - 2 * chunks) * (kPlaceThreads / 32) + warp, steps, lane);
+    return;
+  }
   after_prior();
-  const int which = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int which = blockIdx.x & 1, chunk = blockIdx.x >> 1;
   const uint8_t* counts = a.counts + static_cast<int64_t>(which) * a.items_pad;
-  const int i0 = blockIdx.x * kPlaceItems, mine = i0 + threadIdx.x;
+  const int i0 = chunk * kPlaceItems, mine = i0 + threadIdx.x;
   const int count = threadIdx.x < kPlaceItems && mine < a.items ? counts[mine] : 0;
   const int2 page = threadIdx.x < kPlaceItems && (count & kItemFull) ? a.pages[mine] : make_int2(0, 0);
   int before = 0;
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(kPlaceThreads) append_place_kernel(const __gri
     s_off[threadIdx.x] = off;
     if (count & kItemFull) a.rowoff[which][page.x] = off;
     // (may exceed the capacity: the caller grows the pool before it calls)
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *a.cnt[which] = off + total;
+    if (chunk == chunks - 1 && threadIdx.x == 0) *a.cnt[which] = off + total;
   }
   __syncthreads();
   const int q = lane & 15, th = lane >> 4;
@@ -576,10 +579,10 @@ int row_steps(const exk_append& t, int heads, int sms) {
   return static_cast<int64_t>(t.N) * steps > int64_t{48} * sms ? steps : 1;
 }
 
-int64_t row_blocks(const exk_append& t, int heads, int steps) {
+int64_t row_blocks(const exk_append& t, int heads, int steps, int warps) {
   const int quads = t.q_norm != nullptr ? kQuads<true> : kQuads<false>;
   const int64_t work = static_cast<int64_t>(t.N) * ((heads + 4 * quads * steps - 1) / (4 * quads * steps));
-  return (work + kRowWarps - 1) / kRowWarps;
+  return (work + warps - 1) / warps;
 }
 
 int64_t page_slots(const exk_append& t) {
@@ -601,7 +604,7 @@ extern "C" int exk_rope_append_bf16(const exk_append* t, uint16_t* k_pool, uint1
   int sms = 0;
   if ((r = use_device(device, &sms)) != 0) return r;
   const int heads = t->Hq + 2 * t->Hkv, steps = row_steps(*t, heads, sms);
-  const int64_t blocks = row_blocks(*t, heads, steps);
+  const int64_t blocks = row_blocks(*t, heads, steps, kRowWarps);
   if (blocks >= (int64_t{1} << 31)) return EXK_EARG;
   Append a = {};
   a.t = *t;
@@ -667,16 +670,17 @@ extern "C" int exk_rope_append_compressed(const exk_append* t, const exk_cview* 
   a.pages = reinterpret_cast<int2*>(a.counts + 2 * static_cast<int64_t>(a.items_pad));
   a.status = status;
   const int64_t enc = (2 * items + kRowWarps - 1) / kRowWarps;
+  const int64_t chunks = (items + kPlaceItems - 1) / kPlaceItems;
   const int steps = row_steps(*t, t->Hq, sms);
-  const int64_t blocks = enc + row_blocks(*t, t->Hq, steps);
+  const int64_t blocks = 2 * chunks + row_blocks(*t, t->Hq, steps, kPlaceThreads / 32);
   if (blocks >= (int64_t{1} << 31)) return EXK_EARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool norm = t->q_norm != nullptr;
   const auto encode = norm ? append_encode_kernel<true> : append_encode_kernel<false>;
-  encode<<<static_cast<unsigned>(blocks), kRowWarps * 32, 0, st>>>(a, static_cast<int>(enc), steps);
+  encode<<<static_cast<unsigned>(enc), kRowWarps * 32, 0, st>>>(a);
   if ((r = launch_status()) != 0) return r;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((items + kPlaceItems - 1) / kPlaceItems), 2);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kPlaceThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -684,7 +688,8 @@ extern "C" int exk_rope_append_compressed(const exk_append* t, const exk_cview* 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, norm ? append_place_kernel<true> : append_place_kernel<false>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, norm ? append_place_kernel<true> : append_place_kernel<false>, a,
+                                           static_cast<int>(chunks), steps);
   if (e == cudaSuccess) return 0;
   (void)cudaGetLastError();
   return static_cast<int>(e);
