@@ -315,6 +315,7 @@ __device__ __forceinline__ uint32_t cycles() {
   return t;
 }
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  if (mbar_try_wait(bar, parity)) return true;
   const uint32_t t0 = cycles();
   while (!mbar_try_wait(bar, parity)) {
     if (cycles() - t0 > kWaitCycles) *stop = 1;
@@ -361,8 +362,8 @@ constexpr int kPrefillSmem = 2 * kOperand + kSlots * kOperand + kStage + static_
 static_assert(kPrefillSmem <= 227 * 1024, "one CTA's shared memory");
 
 // The softmax threads' side of one item: query tile x, a row per thread; rt: the
-// row's token in the tile. s_phase:
-// tiles of S this thread has taken so far.
+// row's token in the tile. s_phase, o_phase: tiles of S taken and items ended so
+// far.
 __device__ __forceinline__ void softmax_item(const PrefillArgs& a, const Work& w, Bars* bars, uint32_t tmem, int x, int rt,
                                              uint32_t& s_phase, uint32_t& o_phase, volatile int* stop) {
   const int warp = threadIdx.x >> 5, r = threadIdx.x & 127;
@@ -1037,6 +1038,7 @@ int check_prefill(const exk_prefill* p) {
       p->N > (1 << 28) || p->B > (1 << 24) || p->Hq > 4096)
     return EXK_EARG;
   if (p->Hq / p->Hkv > 16) return EXK_EHEADS;
+  if (prefill_slots(p->N, p->B, p->Hq / p->Hkv) > 65535) return EXK_EARG;  // the grid's second dimension
   if (p->ns > 1 && (p->po == nullptr || p->pm == nullptr || p->pl == nullptr)) return EXK_EARG;
   if (!aligned16(p->q) || !aligned16(p->out) || !aligned16(p->po)) return EXK_EALIGN;
   for (int64_t s : {p->q_st, p->q_sh, p->o_st, p->o_sh})
@@ -1097,7 +1099,6 @@ int launch_prefill(const exk_prefill* p, PrefillArgs& a, const uint16_t* k, int6
   a.ns = p->ns;
   a.scale = p->qk_scale;
   const int64_t slots = prefill_slots(p->N, p->B, a.G);
-  if (slots > 65535) return EXK_EARG;  // over 65,000 blocks of 256 / G tokens
   const dim3 grid(static_cast<unsigned>(p->Hkv * p->ns), static_cast<unsigned>(slots));
   a.by_block = (uint64_t{1} << 36) / static_cast<uint64_t>(2 * a.tpt) + 1;
   a.slots = static_cast<int>(slots);

@@ -691,8 +691,8 @@ def attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None):
     cu_seqlens_k[b] .. (default cu_seqlens) of k and v. A sequence's last query
     sees its last key, so with more keys than queries each query sees the
     excess as context; a query that sees no key gives zeros. Up to 16 query
-    heads per KV head. Returns bf16 [N, Hq, 128]; rows past cu_seqlens[B] are
-    left as they were."""
+    heads per KV head. Returns bf16 [N, Hq, 128] (`out`, which may be q); rows
+    past cu_seqlens[B] are left as they were."""
     if k.dim() != 3 or k.shape[0] == 0 or k.shape[1] == 0:
         raise ValueError("k and v must be [Nk, Hkv, 128] with at least one row")
     Nk, Hkv = k.shape[:2]

@@ -338,6 +338,54 @@ def test_repeat_and_other_stream_give_the_same_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,klens", [([300, 77, 1], [300, 77, 1]), ([5], [6000])])
+def test_output_over_the_queries(lens, klens):
+    """out = q: a block's queries are read before its rows are written (with splits,
+    before the merge writes them)."""
+    q, k, v = inputs(sum(lens), sum(klens), 8, 2, seed=100)
+    cu, ck = offsets(lens).cuda(), offsets(klens).cuda()
+    want = ekv.attention_prefill(q, k, v, cu, ck)
+    own = q.clone()
+    assert ekv.attention_prefill(own, k, v, cu, ck, out=own) is own
+    assert same_bits(own, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("one_stream", [True, False])
+def test_calls_from_two_threads(one_stream):
+    """Two threads that call at once, on one stream or on their own: every call has its
+    own workspace, so each result is what the call alone gives."""
+    import threading
+    work = []
+    for i in range(2):
+        q, k, v = inputs(12, 5000, 8, 2, seed=110 + i)
+        kk, vv, kb, vb, kc, vc, table, sl = _pools([700, 333], 2, seed=120 + i)
+        cu, ck = offsets([12]).cuda(), offsets([5000]).cuda()
+        q2, _, _ = inputs(30, 1, 8, 2, seed=130 + i)
+        c2 = offsets([20, 10]).cuda()
+        want = (ekv.attention_prefill(q, k, v, cu, ck), ekv.attention_prefill_paged(q2, kc, vc, table, sl, c2))
+        work.append(((q, k, v, cu, ck), (q2, kc, vc, table, sl, c2), want, []))
+    torch.cuda.synchronize()
+    shared = torch.cuda.Stream()
+
+    def run(args, pargs, want, bad):
+        with torch.cuda.stream(shared if one_stream else torch.cuda.Stream()):
+            for _ in range(60):
+                a, b = ekv.attention_prefill(*args), ekv.attention_prefill_paged(*pargs)
+                if not (same_bits(a, want[0]) and same_bits(b, want[1])):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not any(w[3] for w in work)
+    kernels.check_status()
+
+
+@pytest.mark.gpu
 def test_prefill_of_one_token_agrees_with_decode_attention():
     """One query per sequence: the decode kernel's result within both bounds."""
     Hq, Hkv, klens = 32, 8, [1000, 513, 260]

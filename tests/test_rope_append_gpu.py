@@ -218,6 +218,45 @@ def test_many_sequences_and_rows_before_the_first():
 
 
 @pytest.mark.gpu
+def test_appends_from_two_threads_on_one_stream():
+    """Two threads append to pools of their own on one stream, their calls' launches
+    interleaved as they come: each call's scratch is its own."""
+    import threading
+    models = [Model(3, 2, 40, seed=20 + i) for i in range(2)]
+    steps = [[[200, 37, 5], [100, 300, 17], [1, 1, 1], [31, 15, 40]], [[16, 0, 90], [7, 333, 1], [40, 41, 42], [1, 2, 3]]]
+    data = [[tokens(sum(new), 4, 2, seed=500 + 50 * i + 3 * j) for j, new in enumerate(s)] for i, s in enumerate(steps)]
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def run(i):
+        m, lens = models[i], [0, 0, 0]
+        with torch.cuda.stream(stream):
+            for new, (q, k, v) in zip(steps[i], data[i]):
+                lens = [a + b for a, b in zip(lens, new)]
+                ekv.rope_append_paged(q, k, v, m.cs, m.kc, m.vc, m.table, ints(lens), offsets(new))
+                ekv.rope_append_reference_paged(q, k, v, m.cs, m.kb, m.vb, m.table, ints(lens), offsets(new))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    kernels.check_status()
+    for m, s, d in zip(models, steps, data):
+        lens = [0, 0, 0]
+        for new, (q, k, v) in zip(s, d):
+            at = 0
+            for b, n in enumerate(new):
+                m.k[b] = torch.cat([m.k[b], rotated(k[at:at + n], m.cs[lens[b]:lens[b] + n])])
+                m.v[b] = torch.cat([m.v[b], v[at:at + n].cpu()])
+                m._count(b, lens[b], lens[b] + n)
+                lens[b] += n
+                at += n
+        m.check()
+
+
+@pytest.mark.gpu
 def test_norm_before_the_rotation():
     Hq, Hkv, new, start = 12, 4, [40, 1, 3], [3, 15, 0]
     g = torch.Generator(device="cuda").manual_seed(1)
@@ -481,7 +520,8 @@ def test_entry_points_refuse_before_any_launch():
         p = PREFILL.pack(*{**pfits, **{n: v or 0 for n, v in kw.items()}}.values())
         return lib.exk_attention_prefill(p, at, 256, 128, at, 256, 128, 4, at, None, 0, None)
 
-    for kw in (dict(q=None), dict(B=0), dict(Hq=7), dict(ns=0), dict(ns=2), dict(q_st=0), dict(cu_q=None)):
+    for kw in (dict(q=None), dict(B=0), dict(Hq=7), dict(ns=0), dict(ns=2), dict(q_st=0), dict(cu_q=None),
+               dict(ns=65), dict(B=65536), dict(N=65535 * 64)):
         assert pre(**kw) == -1, kw
     assert pre(Hq=34, Hkv=2) == -5 and pre(q_sh=132) == -2 and pre(out=at + 8) == -2
     assert lib.exk_prefill_splits(2, 1, 8, 2, 9000, 148) > 1 and lib.exk_prefill_splits(9000, 1, 8, 2, 9000, 148) == 1
