@@ -326,7 +326,8 @@ __device__ __forceinline__ Item load_item(const Append& a, int item, int lane) {
     return it;
   }
   it.pg = it.s.start / kP + (t.cu_seqlens == nullptr ? 0 : slot - (it.s.first / kP + 2 * b));
-  if (it.pg > last_page(it.s) || !tail_of(a, b, it.slot)) return it;
+  // (before the first page: offsets that do not ascend, whose slots are not the sequence's)
+  if (it.pg < it.s.start / kP || it.pg > last_page(it.s) || !tail_of(a, b, it.slot)) return it;
   it.full = (it.pg + 1) * kP <= it.s.start + it.s.n;
   it.later = !it.full && it.pg * kP > it.s.start && it.s.start % kP != 0;
   it.pool = pool_page(a, b, it.pg);

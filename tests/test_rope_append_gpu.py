@@ -351,6 +351,30 @@ def test_positions_and_pages_out_of_range_are_not_stored():
 
 
 @pytest.mark.gpu
+def test_offsets_that_do_not_ascend_stay_in_their_sequences_pages():
+    """With offsets 0, 0, 736, 1000, 0 the page slots of sequence 2 begin at 736 / 16 +
+    4 = 50, but two ends (2 and 8) lie before slots 8 to 49 as well: taken for its
+    pages they would be pages -42 to -1, the last 42 of sequence 1's table row."""
+    new, Hkv = [0, 736, 264, 0], 2
+    q, k, v = tokens(1000, 4, Hkv, seed=97)
+    m = Model(4, Hkv, 64, seed=15)
+    cu = ints([0, 0, 736, 1000, 0])
+    for c in (m.kc, m.vc):
+        c.sm.fill_(7), c.code.fill_(7), c.rowmask.fill_(7), c.base.fill_(7)
+    m.kb.fill_(7.0), m.vb.fill_(7.0)
+    ekv.rope_append_paged(q, k, v, m.cs, m.kc, m.vc, m.table, ints(new), cu)
+    ekv.rope_append_reference_paged(q, k, v, m.cs, m.kb, m.vb, m.table, ints(new), cu)
+    kernels.check_status()
+    theirs = torch.cat([m.table[b, :-(-n // 16)] for b, n in enumerate(new)]).long()
+    other = torch.ones(m.pages, dtype=torch.bool, device="cuda")
+    other[theirs] = False
+    for c, bf in ((m.kc, m.kb), (m.vc, m.vb)):
+        assert (c.rowmask[0, other] == 7).all() and (c.base[0, other] == 7).all()
+        assert (c.sm.view(m.pages, -1)[other] == 7).all() and (c.code.view(m.pages, -1)[other] == 7).all()
+        assert (bf.view(m.pages, -1)[other] == 7).all()
+
+
+@pytest.mark.gpu
 def test_full_raw_pool_drops_rows_past_its_capacity():
     """Slots past the capacity are not written: nothing beyond the pool changes, and
     the counter tells how many rows wanted one. A value far below its page's in
