@@ -232,7 +232,7 @@ __device__ __forceinline__ void load_seq(const PrefillArgs& a, int b, Batch& s) 
   } else {
     s.krow = b * a.k_stride;
     const int most = a.block_table != nullptr ? a.max_pages * kP : a.k_stride, L = __ldg(a.lens + b);
-    if (L > most) set_status(a.status, EXK_S_POSITION);  // keys past the table or the workspace are not seen
+    if (L > most && s.n > 0) set_status(a.status, EXK_S_POSITION);  // keys past the table or the workspace are not seen
     s.L = max(0, min(L, most));
   }
 }
@@ -950,10 +950,12 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constan
 }
 
 // Coded pages of the sequences into bf16 rows b * k_stride + position: the
-// pages' keys (blockIdx.y 0) and values (1), a warp per (page, KV head).
+// pages' keys (blockIdx.y 0) and values (1), a warp per (page, KV head). Nothing
+// of a sequence that has no queries in the call.
 struct Unpack {
   exk_cview c[2];
   uint16_t* out[2];
+  const int32_t* cu_q;
   const int32_t* block_table;
   const int32_t* lens;
   int32_t* status;
@@ -971,7 +973,7 @@ __global__ void __launch_bounds__(256) unpack_kernel(const __grid_constant__ Unp
   const int64_t b = ph / (static_cast<int64_t>(u.Hkv) * u.pages);
   if (b >= u.B) return;
   const int L = min(__ldg(u.lens + b), static_cast<int>(u.k_stride)) - pg * kP;  // rows of the page that are wanted
-  if (L <= 0) return;
+  if (L <= 0 || __ldg(u.cu_q + b + 1) <= __ldg(u.cu_q + b)) return;
   const int pool = __ldg(u.block_table + b * u.max_pages + pg);
   const exk_cview& v = u.c[blockIdx.y];
   const int c = lane & 7, r4 = lane >> 3;
@@ -1240,6 +1242,7 @@ extern "C" int exk_attention_prefill_paged_compressed(const exk_prefill* p, cons
   u.c[1] = *v;
   u.out[0] = k_rows;
   u.out[1] = v_rows;
+  u.cu_q = p->cu_q;
   u.block_table = block_table;
   u.lens = seq_lens;
   u.status = status;

@@ -739,7 +739,8 @@ def attention_prefill_paged(q, kc, vc, block_table, seq_lens, cu_seqlens, max_le
     seq_lens[b] tokens whose pages block_table names, as rope_append_paged left
     them. max_len (host, at least every seq_lens[b]; default max_pages * 16)
     bounds the workspace of B * max_len decoded rows; a longer sequence is cut
-    and reported by check_status(). Bit-identical to
+    and reported by check_status(). Sequences without queries in the call are
+    not read, whatever their lengths and pages. Bit-identical to
     attention_prefill_reference_paged for the same values and max_len."""
     kv, H, pages, _, _ = _coded_pool(kc, q.device, False)
     vv, vH, v_pages, _, _ = _coded_pool(vc, q.device, False)

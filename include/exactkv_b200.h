@@ -398,7 +398,7 @@ int exk_attention_prefill(const exk_prefill *a, const uint16_t *k, int64_t k_st,
  * first seq_lens[b] tokens (its queries' own among them) in the pages that
  * row b of block_table [B, max_pages] names. An entry outside the pool reads
  * as zeros (EXK_S_PAGE_INDEX); a length past the table is cut to it
- * (EXK_S_POSITION). */
+ * (EXK_S_POSITION). Nothing is read of a sequence without queries in the call. */
 int exk_attention_prefill_paged(const exk_prefill *a, const uint16_t *k, const uint16_t *v, int pool_pages,
                                 const int32_t *block_table, int max_pages, const int32_t *seq_lens,
                                 int32_t *status, int device, void *stream);

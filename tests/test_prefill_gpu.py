@@ -241,6 +241,23 @@ def test_lengths_past_the_table_or_the_workspace_are_cut_and_reported():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("idle", [1, 40])
+def test_sequences_without_queries_are_not_read(idle):
+    """Sequences that bring no query may have any length and any pages: the others'
+    results are the same and nothing is reported."""
+    lens, klens = [5] + [0] * idle + [7], [40] + [100] * idle + [64]
+    q, _, _ = inputs(12, 1, 8, 2, seed=35)
+    k, v, kb, vb, kc, vc, table, sl = _pools(klens, 2, seed=36)
+    cu = offsets(lens).cuda()
+    table[1:-1], sl[1:-1] = -9, 1 << 20
+    for call, a, b in ((ekv.attention_prefill_reference_paged, kb, vb), (ekv.attention_prefill_paged, kc, vc)):
+        out = call(q, a, b, table, sl, cu, max_len=64)
+        kernels.check_status()
+        check(out[:5], q[:5], k[:40], v[:40], [5], [40])
+        check(out[5:], q[5:], k[-64:], v[-64:], [7], [64])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("pad", [0, 3])
 def test_many_sequences(pad):
     """More sequences than a warp holds (the other way to map blocks), some empty,
