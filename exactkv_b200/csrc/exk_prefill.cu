@@ -24,6 +24,7 @@
 // TFLOP/s); 4,096: 133 us; 16 prompts of 73 to 1,988 tokens, 28 over 4: 192 us.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "exk_device.cuh"
 #include "exk_encode.cuh"
@@ -1158,15 +1159,29 @@ extern "C" int exk_prefill_splits(int N, int B, int Hq, int Hkv, int64_t max_key
   if (items == 0 || items >= 4 * static_cast<int64_t>(num_sms)) return 1;
   const double row_bytes = static_cast<double>(N) * Hq * (kD + 2) * 4;  // of one split's partials
   if (B > 1) {
-    // As many as fill the SMs once; where the partials are few (16 MB: under 3 us)
-    // twice, since the lengths may differ: 16 sequences of 2 to 8 tokens over
-    // 1,000 to 4,000 keys 109 us, unsplit 115 us. (Splits for the longest
-    // sequences alone, cut to an SM's share on the device, measured slower: 4
-    // sequences of 168 to 484 tokens over 2,600 to 7,500 keys 153 us for 141.)
-    int64_t ns = num_sms / items;
-    const int64_t twice = (2 * static_cast<int64_t>(num_sms) + items - 1) / items;
-    if (twice * row_bytes <= 16e6) ns = twice;
-    return static_cast<int>(std::max<int64_t>(1, std::min(ns, most)));
+    // The lengths are on the device: the queries are taken as spread evenly over the
+    // sequences and the mean length as 0.6 of the longest. A call takes as long as its
+    // longest block or an SM's share (1.8 us a key tile, 4 us a block), and the
+    // partials' traffic and merge. Over 39 shapes (1 to 1,000 queries on 300 to
+    // 28,000 keys, 2 to 64 sequences, packed prompts) within 2 % of the best number
+    // of splits in the mean: 3 sequences of 150 tokens over 4,000 to 15,000 keys 120 us,
+    // unsplit 243; 4 of 168 to 484 over 2,600 to 7,500 unsplit 137 us, two splits 150.
+    // (Splits for the longest sequences alone, cut to an SM's share on the device,
+    // measured slower: the latter 153 us.)
+    const double each = static_cast<double>(N) / B, block = 2. * (kTile / (Hq / Hkv));
+    const double blocks = B * std::ceil(each / block) * Hkv;
+    const double mean = std::max(1., (0.6 * static_cast<double>(max_keys) - 0.5 * each) / kTile);
+    double best = 0.;
+    int64_t choice = 1;
+    for (int64_t ns = 1; ns <= most; ++ns) {
+      double us = std::max(1.8 * static_cast<double>((tiles + ns - 1) / ns) + 4., blocks * (1.8 * mean + 4. * ns) / num_sms);
+      if (ns > 1) us += 6. + 4. * row_bytes * ns / 6.5e6;
+      if (ns == 1 || us < best) {
+        best = us;
+        choice = ns;
+      }
+    }
+    return static_cast<int>(choice);
   }
   // One sequence: its blocks see max_keys - N keys of context and up to N more. The
   // estimate counts waves of blocks (1.8 us a key tile, 4 us a block) where the

@@ -698,9 +698,8 @@ def attention_prefill(q, k, v, cu_seqlens, cu_seqlens_k=None, out=None):
     Nk, Hkv = k.shape[:2]
     k_at, k_st, k_sh = _rows(k, "k", Nk, Hkv, q.device)
     v_at, v_st, v_sh = _rows(v, "v", Nk, Hkv, q.device)
-    # (the plan only: the lengths are on the device, a sequence has about Nk / B keys)
-    many = max(1, cu_seqlens.numel() - 1)
-    a, out, N, B, ws = _prefill_args(q, cu_seqlens, Hkv, Nk if many == 1 else min(Nk, 2 * Nk // many), out)
+    # (the plan only: the lengths are on the device, a sequence has Nk / B keys in the mean)
+    a, out, N, B, ws = _prefill_args(q, cu_seqlens, Hkv, -(-Nk // max(1, cu_seqlens.numel() - 1)), out)
     if cu_seqlens_k is None:
         if Nk != N:
             raise ValueError("k and v rows differ from q's: give cu_seqlens_k")
