@@ -287,10 +287,14 @@ class PagedCompressedKV:
         """Before `tokens` more tokens are appended: one sync to read the slot counter,
         then grow so that even `tokens` tokens of nothing but raw rows fit (they and
         the rows already in open pages: 16 for each sequence). Returns True when the
-        pool moved (a captured graph must be captured again)."""
+        pool moved (a captured graph must be captured again). Raises RuntimeError when
+        appends have wanted more raw rows than there were: the pages that had no room
+        are lost (readers report them) and their sequences must be appended again."""
         used = int(self.cnt.item())
         need = used + (tokens + P * self.pool.nseq) * self.H
         old = self.pool.cap
+        if used > old:
+            raise RuntimeError(f"{used} raw rows appended to a pool of {old}: pages without room were not kept")
         if need <= old:
             return False
         self.pool.enlarge(used, need)

@@ -292,6 +292,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) append_bf16_kernel(const __gri
 // second kernel also writes the sequence's open page.
 constexpr int kItemFull = 0x20, kItemOpens = 0x40, kItemRows = 0x1F;
 
+// rowoff of a page whose raw rows do not all have a slot below the capacity: no
+// row's index (rowoff + rank) is one, so readers report the page. The slots behind
+// the capacity are other sequences' open pages.
+constexpr int kNoRoom = -kP;
+
 struct Item {
   Seq s;
   int h, pg, pool;     // KV head, page of the sequence, its page in the pool (-1: nothing to do)
@@ -504,7 +509,10 @@ __global__ void __launch_bounds__(kPlaceThreads) append_place_kernel(const __gri
       total += i >= threadIdx.x ? n : 0;
     }
     s_off[threadIdx.x] = off;
-    if (count & kItemFull) a.rowoff[which][page.x] = off;
+    if (count & kItemFull) {
+      const int n = count & kItemRows;
+      a.rowoff[which][page.x] = n > 0 && static_cast<int64_t>(off) + n > a.cap[which] ? kNoRoom : off;
+    }
     // (may exceed the capacity: the caller grows the pool before it calls)
     if (chunk == chunks - 1 && threadIdx.x == 0) *a.cnt[which] = off + total;
   }

@@ -619,7 +619,8 @@ def rope_append_paged(q, k, v, cos_sin, kc, vc, block_table, seq_lens, cu_seqlen
     q_norm, k_norm (bf16 [128], both or neither): RMS norm per head first.
     Pages that fill are encoded; each sequence's last, unfilled page stays raw
     in tail slot slots[b] (default b). The caller keeps (N + 15 * B) * Hkv
-    raw rows free (PagedCompressedKV.ensure_headroom(N)). Returns the rotated
+    raw rows free (PagedCompressedKV.ensure_headroom(N)); where they run out, cnt
+    exceeds cap and readers report the pages that had no room. Returns the rotated
     queries [N, Hq, 128] (q_out, which may be q). Positions or pages out of
     range are not stored and reported by check_status()."""
     kv, H, pages, k_cap, k_cnt = _coded_pool(kc, q.device, True)

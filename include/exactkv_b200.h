@@ -352,7 +352,9 @@ int exk_rope_append_bf16(const exk_append *a, uint16_t *k_pool, uint16_t *v_pool
  * exk_encode_pages does, their raw rows taking slots *cnt, *cnt + 1, ... in
  * (sequence, page, head) order; slots at or past cap are not written, so the
  * caller keeps cap - *cnt at least (N + 15 * B) * Hkv before the call (new
- * rows, and those of the open pages that it completes). A page left open holds its
+ * rows, and those of the open pages that it completes). *cnt > cap afterwards: a
+ * page whose raw rows do not all have a slot gets rowoff -16, which readers report
+ * (EXK_S_RAW_INDEX) and read as zeros. A page left open holds its
  * rows raw in the sequence's tail rows, raw[cap + (slots[b] * Hkv + h) * 16,
  * + 16) (rowmask 0xFFFF), where the next call finds them. No page and no tail
  * slot may belong to two sequences of a call that write to it. `scratch`:
