@@ -9,7 +9,7 @@ from .attention import decode_attention
 from .codec import encode_reference, decode_reference, bits_per_value
 from .kernels import attention_compressed, attention_reference, decode_to_bf16, encode_pages
 from .kernels import attention_prefill, attention_prefill_paged, attention_prefill_reference_paged
-from .kernels import rope_append_paged, rope_append_reference_paged, rope_table
+from .kernels import rope_append_paged, rope_append_reference_paged, rope_table, cut_back_paged
 from . import kernels
 
 __version__ = "0.1.0"
@@ -17,7 +17,7 @@ __all__ = ["CompressedKV", "BF16KV", "PagedCompressedKV", "check_overflow", "dec
            "encode_reference", "decode_reference", "bits_per_value",
            "attention_compressed", "attention_reference", "decode_to_bf16", "encode_pages",
            "attention_prefill", "attention_prefill_paged", "attention_prefill_reference_paged", "rope_append_paged",
-           "rope_append_reference_paged", "rope_table", "kernels"]
+           "rope_append_reference_paged", "rope_table", "cut_back_paged", "kernels"]
 
 
 def __getattr__(name):

@@ -84,6 +84,8 @@ _SIGNATURES.update({
     "exk_rope_append_scratch": (c_int64, [c_int, c_int, c_int, c_int]),
     "exk_rope_append_compressed": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
                                            c_void_p, c_int64, c_void_p, c_int, c_void_p]),
+    "exk_reopen_pages": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                 c_int64, c_void_p, c_int, c_void_p]),
     "exk_prefill_splits": (c_int, [c_int, c_int, c_int, c_int, c_int64, c_int]),
     "exk_attention_prefill": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int,
                                       c_void_p, c_void_p, c_int, c_void_p]),

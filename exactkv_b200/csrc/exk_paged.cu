@@ -32,7 +32,7 @@ struct Append {
   int32_t* rowmask[2];
   int32_t* rowoff[2];
   uint16_t* raw[2];
-  int64_t cap[2];
+  int64_t cap[2], raw_rows[2];
   int32_t* cnt[2];
   int32_t tails;      // open pages per KV head that the raw pools hold
   uint8_t* counts;    // [2][items_pad] raw rows of every item, and its flags (scratch)
@@ -554,6 +554,76 @@ __global__ void __launch_bounds__(kPlaceThreads) append_place_kernel(const __gri
   }
 }
 
+// ---------------------------------------------------------------- sequences cut back
+//
+// A sequence whose length was taken back (drafts that were not accepted) may end
+// inside a page that was completed: its rows are coded, and the tail rows, where the
+// next append looks for the page's earlier rows, hold a later page's. A warp per
+// (sequence, KV head) of the keys and of the values: the page's remaining rows,
+// decoded (all loaded before the first is), go to the tail rows, and the page is
+// open again. Pages that are open, and ends of whole pages, are left alone: the look
+// is all that most calls cost (64 sequences of 8 heads: 2.2 us; all reopened 4.0).
+
+__global__ void __launch_bounds__(kRowWarps * 32) reopen_kernel(const __grid_constant__ Append a) {
+  const exk_append& t = a.t;
+  const int lane = threadIdx.x & 31, q = lane & 15, th = lane >> 4;
+  const int work = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (work >= 2 * a.items) return;
+  const int which = work >= a.items ? 1 : 0, item = work - which * a.items;
+  const int b = item / t.Hkv, h = item % t.Hkv, len = __ldg(t.seq_lens + b), held = len % kP;
+  if (len <= 0 || held == 0) return;
+  if (len > t.max_pages * kP) {
+    set_status(a.status, EXK_S_POSITION);
+    return;
+  }
+  int slot;
+  if (!tail_of(a, b, slot)) return;
+  const int pool = pool_page(a, b, len / kP);
+  if (pool < 0) return;
+  const int64_t page = static_cast<int64_t>(pool) * t.Hkv + h;
+  const int64_t tail = a.cap[which] + (static_cast<int64_t>(slot) * t.Hkv + h) * kP;
+  const uint32_t rm = static_cast<uint32_t>(a.rowmask[which][page]) & 0xFFFFu;
+  const int32_t ro = a.rowoff[which][page];
+  if (rm == 0xFFFFu && ro == tail) return;
+  const int n = min(held - 8 * th, 8);
+  const uint32_t bl = *reinterpret_cast<const uint32_t*>(a.base[which] + page * kD + 4 * q);
+  const uint32_t bh = *reinterpret_cast<const uint32_t*>(a.base[which] + page * kD + 64 + 4 * q);
+  uint32_t w[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 8 * th + i;
+    const int64_t row = (static_cast<int64_t>(pool) * kP + r) * t.Hkv + h;
+    const int64_t ridx = static_cast<int64_t>(ro) + __popc(rm & ((1u << r) - 1u));
+    w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0u;
+    if (i >= n) continue;
+    if (((rm >> r) & 1u) == 0u) {
+      w[i][0] = *reinterpret_cast<const uint32_t*>(a.sm[which] + row * kD + 4 * q);
+      w[i][1] = *reinterpret_cast<const uint32_t*>(a.sm[which] + row * kD + 64 + 4 * q);
+      w[i][2] = *reinterpret_cast<const uint32_t*>(a.code[which] + row * (kD / 2) + 4 * q);
+    } else if (ridx >= 0 && ridx < a.raw_rows[which]) {
+      const uint16_t* src = a.raw[which] + ridx * kD;
+      const uint2 lo = *reinterpret_cast<const uint2*>(src + 4 * q), hi = *reinterpret_cast<const uint2*>(src + 64 + 4 * q);
+      w[i][0] = lo.x; w[i][1] = lo.y; w[i][2] = hi.x; w[i][3] = hi.y;
+    } else {
+      set_status(a.status, EXK_S_RAW_INDEX);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i >= n) break;
+    if (((rm >> (8 * th + i)) & 1u) == 0u) {
+      const uint32_t sl = w[i][0], sh = w[i][1], cw = w[i][2];
+      dec4(sl, lo_nibbles(cw), bl & 0x7F7F7F7Fu, bl, w[i][0], w[i][1]);
+      dec4(sh, hi_nibbles(cw), bh & 0x7F7F7F7Fu, bh, w[i][2], w[i][3]);
+    }
+    store_quads(tail_row(a, which, slot, h, 8 * th + i), q, w[i]);
+  }
+  if (lane == 0) {
+    a.rowmask[which][page] = 0xFFFF;
+    a.rowoff[which][page] = static_cast<int32_t>(tail);
+  }
+}
+
 }  // namespace exk
 
 using namespace exk;
@@ -592,6 +662,34 @@ int64_t row_blocks(const exk_append& t, int heads, int steps, int warps) {
   const int quads = t.q_norm != nullptr ? kQuads<true> : kQuads<false>;
   const int64_t work = static_cast<int64_t>(t.N) * ((heads + 4 * quads * steps - 1) / (4 * quads * steps));
   return (work + warps - 1) / warps;
+}
+
+// The pools of a call whose a.t is set, checked.
+int coded_pools(Append& a, const exk_cview* k, int64_t k_cap, const exk_cview* v, int64_t v_cap) {
+  if (k->sm == v->sm || k->raw == v->raw) return EXK_EARG;  // keys and values have pools of their own
+  const exk_cview* c[2] = {k, v};
+  const int64_t cap[2] = {k_cap, v_cap};
+  int64_t tails = int64_t{1} << 24;
+  for (int i = 0; i < 2; ++i) {
+    if (c[i]->sm == nullptr || c[i]->code == nullptr || c[i]->base == nullptr || c[i]->rowmask == nullptr ||
+        c[i]->rowoff == nullptr || c[i]->raw == nullptr || cap[i] < 0 || c[i]->raw_rows < cap[i] ||
+        c[i]->raw_rows >= (int64_t{1} << 31))
+      return EXK_EARG;
+    if (!aligned16(c[i]->sm) || !aligned16(c[i]->code) || !aligned16(c[i]->base) || !aligned16(c[i]->raw))
+      return EXK_EALIGN;
+    tails = std::min(tails, (c[i]->raw_rows - cap[i]) / (static_cast<int64_t>(a.t.Hkv) * kP));
+    a.sm[i] = const_cast<uint8_t*>(c[i]->sm);
+    a.code[i] = const_cast<uint8_t*>(c[i]->code);
+    a.base[i] = const_cast<uint8_t*>(c[i]->base);
+    a.rowmask[i] = const_cast<int32_t*>(c[i]->rowmask);
+    a.rowoff[i] = const_cast<int32_t*>(c[i]->rowoff);
+    a.raw[i] = const_cast<uint16_t*>(c[i]->raw);
+    a.cap[i] = cap[i];
+    a.raw_rows[i] = c[i]->raw_rows;
+  }
+  if (tails < (a.t.slots == nullptr ? a.t.B : 1)) return EXK_EARG;  // an open page for every sequence
+  a.tails = static_cast<int32_t>(tails);
+  return 0;
 }
 
 int64_t page_slots(const exk_append& t) {
@@ -637,40 +735,20 @@ extern "C" int exk_rope_append_compressed(const exk_append* t, const exk_cview* 
   int r = check_append(t);
   if (r != 0) return r;
   if (k == nullptr || v == nullptr || k_cnt == nullptr || v_cnt == nullptr || scratch == nullptr) return EXK_EARG;
-  if (k->sm == v->sm || k->raw == v->raw || k_cnt == v_cnt) return EXK_EARG;  // keys and values have pools of their own
-  const exk_cview* c[2] = {k, v};
-  const int64_t cap[2] = {k_cap, v_cap};
-  int32_t* cnt[2] = {k_cnt, v_cnt};
+  if (k_cnt == v_cnt) return EXK_EARG;
   const int64_t items = page_slots(*t) * t->Hkv;
   if (items > (int64_t{1} << 29)) return EXK_EARG;
   Append a = {};
   a.t = *t;
-  int64_t tails = int64_t{1} << 24;
-  for (int i = 0; i < 2; ++i) {
-    if (c[i]->sm == nullptr || c[i]->code == nullptr || c[i]->base == nullptr || c[i]->rowmask == nullptr ||
-        c[i]->rowoff == nullptr || c[i]->raw == nullptr || cap[i] < 0 || c[i]->raw_rows < cap[i] ||
-        c[i]->raw_rows >= (int64_t{1} << 31))
-      return EXK_EARG;
-    if (!aligned16(c[i]->sm) || !aligned16(c[i]->code) || !aligned16(c[i]->base) || !aligned16(c[i]->raw))
-      return EXK_EALIGN;
-    tails = std::min(tails, (c[i]->raw_rows - cap[i]) / (static_cast<int64_t>(t->Hkv) * kP));
-    a.sm[i] = const_cast<uint8_t*>(c[i]->sm);
-    a.code[i] = const_cast<uint8_t*>(c[i]->code);
-    a.base[i] = const_cast<uint8_t*>(c[i]->base);
-    a.rowmask[i] = const_cast<int32_t*>(c[i]->rowmask);
-    a.rowoff[i] = const_cast<int32_t*>(c[i]->rowoff);
-    a.raw[i] = const_cast<uint16_t*>(c[i]->raw);
-    a.cap[i] = cap[i];
-    a.cnt[i] = cnt[i];
-  }
-  if (tails < (t->slots == nullptr ? t->B : 1)) return EXK_EARG;  // an open page for every sequence
+  if ((r = coded_pools(a, k, k_cap, v, v_cap)) != 0) return r;
+  a.cnt[0] = k_cnt;
+  a.cnt[1] = v_cnt;
   if (!aligned16(scratch)) return EXK_EALIGN;
   if (scratch_bytes < exk_rope_append_scratch(t->N, t->B, t->Hkv, t->cu_seqlens != nullptr)) return EXK_EARG;
   if (t->N == 0) return 0;
   DeviceScope scope;
   int sms = 0;
   if ((r = use_device(device, &sms)) != 0) return r;
-  a.tails = static_cast<int32_t>(tails);
   a.slots = static_cast<int32_t>(page_slots(*t));
   a.items = static_cast<int32_t>(items);
   a.items_pad = static_cast<int32_t>((items + 15) / 16 * 16);
@@ -702,4 +780,30 @@ extern "C" int exk_rope_append_compressed(const exk_append* t, const exk_cview* 
   if (e == cudaSuccess) return 0;
   (void)cudaGetLastError();
   return static_cast<int>(e);
+}
+
+extern "C" int exk_reopen_pages(const int32_t* block_table, int B, int max_pages, int pool_pages, int Hkv,
+                                const int32_t* seq_lens, const int32_t* slots, const exk_cview* k, int64_t k_cap,
+                                const exk_cview* v, int64_t v_cap, int32_t* status, int device, void* stream) {
+  if (block_table == nullptr || seq_lens == nullptr || k == nullptr || v == nullptr || B <= 0 || B > (1 << 24) ||
+      max_pages <= 0 || max_pages > (1 << 26) || pool_pages <= 0 || Hkv <= 0 || Hkv > 4096 ||
+      static_cast<int64_t>(pool_pages) * Hkv >= (int64_t{1} << 31) || static_cast<int64_t>(B) * Hkv > (int64_t{1} << 29))
+    return EXK_EARG;
+  Append a = {};
+  a.t.block_table = block_table;
+  a.t.seq_lens = seq_lens;
+  a.t.slots = slots;
+  a.t.B = B;
+  a.t.Hkv = Hkv;
+  a.t.max_pages = max_pages;
+  a.t.pool_pages = pool_pages;
+  int r = coded_pools(a, k, k_cap, v, v_cap);
+  if (r != 0) return r;
+  a.items = B * Hkv;
+  a.status = status;
+  DeviceScope scope;
+  if ((r = use_device(device, nullptr)) != 0) return r;
+  const unsigned blocks = static_cast<unsigned>((2 * static_cast<int64_t>(a.items) + kRowWarps - 1) / kRowWarps);
+  reopen_kernel<<<blocks, kRowWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return launch_status();
 }

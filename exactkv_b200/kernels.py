@@ -618,7 +618,8 @@ def rope_append_paged(q, k, v, cos_sin, kc, vc, block_table, seq_lens, cu_seqlen
     last: positions seq_lens[b] - n_b .. seq_lens[b] - 1. cos_sin: rope_table().
     q_norm, k_norm (bf16 [128], both or neither): RMS norm per head first.
     Pages that fill are encoded; each sequence's last, unfilled page stays raw
-    in tail slot slots[b] (default b). The caller keeps (N + 15 * B) * Hkv
+    in tail slot slots[b] (default b), where the next call looks for it (after a
+    sequence was cut back: cut_back_paged() first). The caller keeps (N + 15 * B) * Hkv
     raw rows free (PagedCompressedKV.ensure_headroom(N)); where they run out, cnt
     exceeds cap and readers report the pages that had no room. Returns the rotated
     queries [N, Hq, 128] (q_out, which may be q). Positions or pages out of
@@ -639,6 +640,30 @@ def rope_append_paged(q, k, v, cos_sin, kc, vc, block_table, seq_lens, cu_seqlen
                                          status_tensor(dev).data_ptr(), dev,
                                          _stream(dev)), "exk_rope_append_compressed")
     return q_out
+
+
+def cut_back_paged(kc, vc, block_table, seq_lens, slots=None):
+    """After sequences of the compressed pools kc, vc were cut back to seq_lens [B]
+    tokens (drafts that were not taken) and before the next rope_append_paged: a
+    page that had been completed and now ends the sequence is opened again, its
+    rows in tail slot slots[b] (default b). Sequences whose last page is open, or
+    whole, are left alone, so every sequence of a step may go through it; one
+    launch, no sync. (bf16 pools need nothing of the kind.)"""
+    dev = block_table.device
+    kv, H, pages, k_cap, _ = _coded_pool(kc, dev, True)
+    vv, vH, v_pages, v_cap, _ = _coded_pool(vc, dev, True)
+    if vH != H or v_pages != pages:
+        raise ValueError("the key and value pools differ in shape")
+    if block_table.dim() != 2 or block_table.shape[1] == 0 or not block_table.is_cuda:
+        raise ValueError("block_table must be a CUDA tensor [B, max_pages]")
+    B, max_pages = block_table.shape
+    table = _index(block_table, "block_table", (B, max_pages), dev)
+    lens = _index(seq_lens, "seq_lens", (B,), dev)
+    at = 0 if slots is None else _index(slots, "slots", (B,), dev)
+    if B == 0:
+        return
+    check(lib.exk_reopen_pages(table, B, max_pages, pages, H, lens, at, kv, k_cap, vv, v_cap,
+                               status_tensor(dev.index).data_ptr(), dev.index, _stream(dev.index)), "exk_reopen_pages")
 
 
 def rope_append_reference_paged(q, k, v, cos_sin, k_pool, v_pool, block_table, seq_lens, cu_seqlens=None, q_norm=None,

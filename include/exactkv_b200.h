@@ -356,7 +356,8 @@ int exk_rope_append_bf16(const exk_append *a, uint16_t *k_pool, uint16_t *v_pool
  * page whose raw rows do not all have a slot gets rowoff -16, which readers report
  * (EXK_S_RAW_INDEX) and read as zeros. A page left open holds its
  * rows raw in the sequence's tail rows, raw[cap + (slots[b] * Hkv + h) * 16,
- * + 16) (rowmask 0xFFFF), where the next call finds them. No page and no tail
+ * + 16) (rowmask 0xFFFF), where the next call finds them (a sequence that was cut
+ * back since: exk_reopen_pages first). No page and no tail
  * slot may belong to two sequences of a call that write to it. `scratch`:
  * exk_rope_append_scratch() bytes (packed: cu_seqlens given), 16-byte
  * aligned, in use until the call has run. Two launches. */
@@ -364,6 +365,17 @@ int64_t exk_rope_append_scratch(int N, int B, int Hkv, int packed);
 int exk_rope_append_compressed(const exk_append *a, const exk_cview *k, int64_t k_cap, int32_t *k_cnt,
                                const exk_cview *v, int64_t v_cap, int32_t *v_cnt, void *scratch,
                                int64_t scratch_bytes, int32_t *status, int device, void *stream);
+
+/* Sequences cut back to seq_lens[b] tokens (drafts that were not taken). Where a
+ * length ends inside a page that an append had completed, exk_rope_append_compressed
+ * would look for the page's rows in the tail rows, which hold another page's: here they
+ * are decoded into the tail rows and the page is open again (in both pools; rowmask
+ * 0xFFFF). Call it after the cut and before the next append; pages that are open and
+ * lengths of whole pages are left alone. Lengths, entries and tail slots out of range
+ * are reported and nothing of the sequence is written. One launch. */
+int exk_reopen_pages(const int32_t *block_table, int B, int max_pages, int pool_pages, int Hkv,
+                     const int32_t *seq_lens, const int32_t *slots, const exk_cview *k, int64_t k_cap,
+                     const exk_cview *v, int64_t v_cap, int32_t *status, int device, void *stream);
 
 /* Causal attention of many query tokens per sequence: N packed queries q [N,
  * Hq, 128] (element strides q_st, q_sh, multiples of 8; 16-byte aligned),

@@ -89,3 +89,121 @@ def test_pages_without_room_in_the_raw_pool_are_refused_by_readers():
     kernels.check_status()
     with pytest.raises(RuntimeError, match="raw rows"):
         m.vc.ensure_headroom(1)
+
+
+# ----------------------------------------------------------------------------- what sequences hold
+
+CUTS = [  # (tokens held, new tokens) of two sequences, call by call: fewer held than the call before left is a cut
+    [(0, 45), (0, 20)],
+    [(45, 5), (20, 14)],       # drafts that complete a page each and open the next
+    [(46, 1), (25, 3)],        # cut back into the completed pages, which stay open
+    [(47, 1), (28, 4)],        # ... and fill again
+    [(48, 20), (32, 40)],
+    [(40, 30), (33, 1)],       # into a page that this call completes before it opens another; by two pages
+    [(5, 3), (34, 60)],
+    [(8, 8), (94, 0)],
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["paged", "contiguous", "slots"])
+@pytest.mark.parametrize("every", [1, 3, 1000])
+def test_sequences_cut_back_into_completed_pages(kind, every):
+    """Rejected drafts: the lengths end inside a page that was completed and coded. Both pools hold the
+    same rows after every cut and every call, and are attended with the same bits; also
+    with a CompressedKV as the pool, and with other tail slots."""
+    Hq, Hkv = 8, 4
+    m = Model(2, Hkv, 8, spare=0, seed=33, tails=5)
+    slots = None
+    if kind == "contiguous":
+        m.kc, m.vc = (ekv.CompressedKV(2, 128, Hkv, D, reserve=2.0) for _ in range(2))
+    else:
+        slots = ints([3, 1]) if kind == "slots" else None
+        for c in (m.kc, m.vc):
+            c.ensure_headroom(2000)
+    for i, call in enumerate(CUTS):
+        lens, new = [h + n for h, n in call], [n for _, n in call]
+        q, k, v = tokens(sum(new), Hq, Hkv, seed=710 + 3 * i)
+        escaping(k, v, every)
+        held = [h for h, _ in call]
+        if i and held != left:
+            ekv.cut_back_paged(m.kc, m.vc, m.table, ints(held), slots)
+            check_same_pools(m, held)
+            before = [t.clone() for c in (m.kc, m.vc) for t in (c.raw, c.rowmask, c.rowoff)]
+            ekv.cut_back_paged(m.kc, m.vc, m.table, ints(held), slots)      # nothing is left to do
+            assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in
+                       zip(before, [t for c in (m.kc, m.vc) for t in (c.raw, c.rowmask, c.rowoff)]))
+        left = lens
+        qr = append_both(m, q, k, v, lens, new, slots)
+        check_same_pools(m, lens)
+        sl, cu = ints(lens), offsets(new)
+        a = ekv.attention_prefill_paged(qr, m.kc, m.vc, m.table, sl, cu)
+        assert same_bits(a, ekv.attention_prefill_reference_paged(qr, m.kb, m.vb, m.table, sl, cu))
+        q1 = torch.randn(2, Hq, D, device="cuda").to(torch.bfloat16)
+        a = kernels.attention_paged(q1, m.kc, m.vc, m.table, sl)
+        assert same_bits(a, kernels.attention_reference_paged(q1, m.kb, m.vb, m.table, sl))
+        kernels.check_status()
+    assert int(m.vc.cnt.item()) > (0 if every == 1000 else 100)
+
+
+@pytest.mark.gpu
+def test_cut_back_in_a_captured_step_and_out_of_range():
+    """Captured: it follows the lengths on the device. Lengths, pages and slots out of
+    range are reported, and nothing of their sequences changes."""
+    Hq, Hkv, B = 4, 2, 3
+    m = Model(B, Hkv, 3, seed=34)
+    q, k, v = tokens(3 * 40, Hq, Hkv, seed=735)
+    escaping(k, v, 2)
+    append_both(m, q, k, v, [40] * 3, [40] * 3)
+    sl = ints([40] * 3)
+    ekv.cut_back_paged(m.kc, m.vc, m.table, sl)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ekv.cut_back_paged(m.kc, m.vc, m.table, sl)
+    bad = m.table.clone()
+    bad[2, 1] = -4
+    for lens, table, slots, match in (([49, 0, -7], m.table, None, "length"), ([40, 40, 20], bad, None, "outside the pool"),
+                                      ([20, 40, 40], m.table, [3, 1, 2], "tail slot")):
+        before = [t.clone() for c in (m.kc, m.vc) for t in (c.raw, c.rowmask, c.rowoff)]
+        ekv.cut_back_paged(m.kc, m.vc, table, ints(lens), None if slots is None else ints(slots))
+        with pytest.raises(RuntimeError, match=match):
+            kernels.check_status()
+        assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in
+                   zip(before, [t for c in (m.kc, m.vc) for t in (c.raw, c.rowmask, c.rowoff)]))
+    lens = [17, 32, 5]
+    sl.copy_(ints(lens))
+    graph.replay()
+    kernels.check_status()
+    check_same_pools(m, lens)
+    q, k, v = tokens(3 * 30, Hq, Hkv, seed=738)
+    lens = [n + 30 for n in lens[:1]] + [lens[1], lens[2] + 4]
+    append_both(m, q[:34], k[:34], v[:34], lens, [30, 0, 4])
+    check_same_pools(m, lens)
+    kernels.check_status()
+
+
+def test_cut_back_refusals():
+    """On the host, before any launch (addresses never touched)."""
+    import ctypes
+    from exactkv_b200._lib import CView, lib
+    at = 1 << 40
+    kc, vc, short = (CView(x, x, x, x, x, x, n) for x, n in ((at, 1000 + 4 * 32), (2 * at, 1000 + 4 * 32), (at, 1000 + 3 * 32)))
+    fits = dict(table=at, B=4, max_pages=4, pages=16, H=2, lens=at, slots=None, k=kc, k_cap=1000, v=vc, v_cap=1000)
+
+    def call(**kw):
+        a = {**fits, **kw}
+        for n in ("k", "v"):
+            a[n] = None if a[n] is None else ctypes.byref(a[n])
+        return lib.exk_reopen_pages(*a.values(), None, 0, None)
+
+    for kw in (dict(table=None), dict(B=0), dict(max_pages=0), dict(pages=0), dict(H=0), dict(lens=None), dict(k=None),
+               dict(v=kc), dict(k=short), dict(k_cap=-1), dict(v_cap=2000), dict(pages=1 << 30, H=4)):
+        assert call(**kw) == -1, kw
+    assert call(k=CView(at + 4, at, at, at, at, at, 1000 + 4 * 32)) == -2
+    pool = ekv.PagedCompressedKV(4, 2, D, 2, device="cpu")
+    for args in ((pool, pool, torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)),
+                 (pool, ekv.PagedCompressedKV(5, 2, D, 2, device="cpu"), torch.zeros(2, 4, dtype=torch.int32),
+                  torch.zeros(2, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            ekv.cut_back_paged(*args)
