@@ -334,7 +334,9 @@ __device__ __forceinline__ Item load_item(const Append& a, int item, int lane) {
   // (before the first page: offsets that do not ascend, whose slots are not the sequence's)
   if (it.pg < it.s.start / kP || it.pg > last_page(it.s) || !tail_of(a, b, it.slot)) return it;
   it.full = (it.pg + 1) * kP <= it.s.start + it.s.n;
-  it.later = !it.full && it.pg * kP > it.s.start && it.s.start % kP != 0;
+  // (where the first page's entry is bad nothing of that page is read or written, and
+  // the open one need not wait for it)
+  it.later = !it.full && it.pg * kP > it.s.start && it.s.start % kP != 0 && pool_page(a, b, it.s.start / kP) >= 0;
   it.pool = pool_page(a, b, it.pg);
   return it;
 }

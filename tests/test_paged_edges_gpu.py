@@ -207,3 +207,26 @@ def test_cut_back_refusals():
                   torch.zeros(2, dtype=torch.int32))):
         with pytest.raises(ValueError):
             ekv.cut_back_paged(*args)
+
+
+@pytest.mark.gpu
+def test_open_page_is_written_beside_a_bad_entry():
+    """A call that would complete a page whose entry is bad and opens another: the good
+    entries' pages hold what the bf16 pool holds."""
+    Hq, Hkv = 4, 2
+    m = Model(1, Hkv, 4, seed=35)
+    q, k, v = tokens(20, Hq, Hkv, seed=740)
+    append_both(m, q, k, v, [20], [20])
+    good = m.table.clone()
+    m.table[0, 1] = m.pages
+    q, k, v = tokens(30, Hq, Hkv, seed=743)
+    append_both(m, q, k, v, [50], [30])
+    with pytest.raises(RuntimeError, match="outside the pool"):
+        kernels.check_status()
+    m.table = good
+    for c, bf in ((m.kc, m.kb), (m.vc, m.vb)):
+        got = decoded(c)
+        for lo, hi in ((0, 16), (32, 48), (48, 50)):
+            r = rows_of(m, 0, hi, lo)
+            assert same_bits(got[r], bf[0][r]), lo
+    kernels.check_status()
