@@ -121,18 +121,28 @@ __device__ __forceinline__ void load_turn(const float* cs, int c0, Turn<NW>& t) 
 
 // One head held by a group of lanes, NW packed words of each half (channels c0 ..
 // c0 + 2 NW - 1 and those + 64) to a lane: this lane's part of its sum of squares.
+// Every path adds in one order, whatever its lanes hold: channels 4i .. 4i + 3 and
+// those + 64 first (i = 0 .. 15), then i with i ^ 1, i ^ 8, i ^ 4 and i ^ 2.
 template <int NW>
 __device__ __forceinline__ float squares(const uint32_t (&lo)[NW], const uint32_t (&hi)[NW]) {
-  F2 ss = f2(0.f, 0.f);
+  float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < NW; ++j) {
-    const F2 x = f2_bf16(lo[j]), y = f2_bf16(hi[j]);
-    ss = fma2(y, y, fma2(x, x, ss));
+  for (int i = 0; i < NW; i += 2) {
+    F2 ss = f2(0.f, 0.f);
+#pragma unroll
+    for (int j = i; j < i + 2; ++j) {
+      const F2 x = f2_bf16(lo[j]), y = f2_bf16(hi[j]);
+      ss = fma2(y, y, fma2(x, x, ss));
+    }
+    float s0, s1;
+    split2(ss, s0, s1);
+    sum = i == 0 ? s0 + s1 : sum + (s0 + s1);
   }
-  float s0, s1;
-  split2(ss, s0, s1);
-  return s0 + s1;
+  return sum;
 }
+
+// 1 / sqrt(mean square + eps) of a head's sum of squares.
+__device__ __forceinline__ float norm_factor(float sum, float eps) { return rsqrtf(fmaf(sum, 1.f / kD, eps)); }
 
 // The head rotated, after the norm by weight w where NORM: r = 1 / sqrt(mean square + eps).
 template <int NW, bool NORM>
@@ -242,7 +252,7 @@ __device__ __forceinline__ void token_rows(const Append& a, int64_t work, int st
         for (int u = 0; u < Q; ++u) r[u] += __shfl_xor_sync(0xFFFFFFFFu, r[u], d);
       }
 #pragma unroll
-      for (int u = 0; u < Q; ++u) r[u] = rsqrtf(r[u] * (1.f / kD) + t.eps);
+      for (int u = 0; u < Q; ++u) r[u] = norm_factor(r[u], t.eps);
     }
 #pragma unroll
     for (int u = 0; u < Q; ++u) {
@@ -369,8 +379,8 @@ __device__ __forceinline__ void cache_form(const Append& a, int which, int pos, 
   if constexpr (NORM) {
     r = squares<2>(l, g);
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) r += __shfl_xor_sync(0xFFFFFFFFu, r, d);
-    r = rsqrtf(r * (1.f / kD) + a.t.eps);
+    for (int d : {1, 8, 4, 2}) r += __shfl_xor_sync(0xFFFFFFFFu, r, d);
+    r = norm_factor(r, a.t.eps);
   }
   norm_rotate<2, NORM>(l, g, 4 * q, a.t.k_norm, r, turn);
   w[0] = l[0]; w[1] = l[1]; w[2] = g[0]; w[3] = g[1];

@@ -230,3 +230,51 @@ def test_open_page_is_written_beside_a_bad_entry():
             r = rows_of(m, 0, hi, lo)
             assert same_bits(got[r], bf[0][r]), lo
     kernels.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[16 * 40] * 32, [13] * 1300, [31] * 520])
+def test_normed_keys_have_the_same_bits_in_both_pools(lens):
+    """Over 1e5 normed heads a pool, in encoded pages, among them raw rows, and in open
+    pages: one order of the sum of squares for every path."""
+    Hkv, B = 8, len(lens)
+    n = sum(lens)
+    m = Model(B, Hkv, -(-max(lens) // 16), seed=37)
+    g = torch.Generator(device="cuda").manual_seed(38)
+    wq, wk = (torch.randn(D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    q, k, v = tokens(n, Hkv, Hkv, seed=750)
+    escaping(k, v, 5)
+    append_both(m, q, k, v, lens, lens, q_norm=wq, k_norm=wk)
+    kernels.check_status()
+    assert n * Hkv >= 100000 and (max(lens) < 16 or int(m.kc.cnt.item()) > 1000)
+    at = torch.cat([rows_of(m, b, m_) for b, m_ in enumerate(lens)])
+    got = decoded(m.kc)
+    assert same_bits(got[at], m.kb[0][at])
+    assert same_bits(decoded(m.vc)[at], v)
+
+
+@pytest.mark.gpu
+def test_normed_keys_and_queries_one_token_at_a_time():
+    """The same bits as the whole prompt gives, and within the norm's bound of the formula."""
+    Hq, Hkv, B, n = 8, 8, 400, 33
+    m, whole = (Model(B, Hkv, 3, seed=39) for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(40)
+    w = dict(zip(("q_norm", "k_norm"), (torch.randn(D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))))
+    q, k, v = tokens(B * n, Hq, Hkv, seed=760)
+    escaping(k, v, 7)
+    qw = append_both(whole, q, k, v, [n] * B, [n] * B, **w).view(B, n, Hq, D)
+    parts = [t.view(B, n, -1, D) for t in (q, k, v)]
+    for i in range(n):
+        one = [t[:, i].contiguous() for t in parts]
+        sl = ints([i + 1] * B)
+        a = ekv.rope_append_paged(*one, m.cs, m.kc, m.vc, m.table, sl, **w)
+        b = ekv.rope_append_reference_paged(*one, m.cs, m.kb, m.vb, m.table, sl, **w)
+        assert same_bits(a, b) and same_bits(a, qw[:, i].contiguous())
+    kernels.check_status()
+    at = torch.cat([rows_of(m, b, n) for b in range(B)])
+    assert same_bits(m.kb, whole.kb)
+    for c in (m.kc, whole.kc):
+        assert same_bits(decoded(c)[at], m.kb[0][at])
+    some = torch.arange(0, B * n, 97)
+    y, tol = rotated(k[some.cuda()], m.cs.cpu()[some % n], w["k_norm"])
+    assert ((m.kb[0][at][some.cuda()].double().cpu() - y).abs() <= tol).all()
