@@ -251,6 +251,13 @@ __device__ __forceinline__ Batch load_batch(const PrefillArgs& a, int lane) {
   return s;
 }
 
+// Offsets of a batch: 0 <= cu[0] <= .. <= cu[B] <= most. By a whole warp, one answer.
+__device__ __forceinline__ bool ascending(const int32_t* cu, int B, int most, int lane) {
+  bool ok = __ldg(cu) >= 0 && __ldg(cu + B) <= most;
+  for (int b = lane; b < B; b += 32) ok = ok && __ldg(cu + b) <= __ldg(cu + b + 1);
+  return __all_sync(0xFFFFFFFFu, ok);
+}
+
 // Block (x, y) of the grid: (KV head, split) and 256-row block of T = 2 tpt tokens,
 // a sequence's blocks with long rows of keys first. With more than 32 sequences,
 // b's blocks take slots cu[b] / T + b, + 1, ...: n tokens need at most (n + T - 1) /
@@ -630,6 +637,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOutput));
     const int rt = (threadIdx.x & 127) / a.G;
     uint32_t o_phase = 0;
+    // (a warp that waits for the first rows anyway)
+    if (warp == 8 && blockIdx.x == 0 && blockIdx.y == 0 &&
+        !(ascending(a.cu_q, a.B, a.N, lane) && (a.cu_k == nullptr || ascending(a.cu_k, a.B, a.Nk, lane))))
+      set_status(a.status, EXK_S_POSITION);
     Work w;
     while (next_work(w))
       for (int x = 0; x < w.tiles; ++x) output_item(a, w, bars, stage, tmem, x, rt, o_phase, stop);
@@ -907,7 +918,8 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constan
   const int lane = threadIdx.x & 31;
   if (row >= static_cast<int64_t>(a.N) * a.Hq) return;
   const int tok = static_cast<int>(row / a.Hq);
-  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.B)) return;
+  // (offsets that are no batch's may name rows whose partials nothing wrote)
+  if (tok < __ldg(a.cu_q) || tok >= __ldg(a.cu_q + a.B) || !ascending(a.cu_q, a.B, a.N, lane)) return;
   float m[2], l[2], f[2];
   float M = -INFINITY, den = 0.f;
 #pragma unroll

@@ -60,7 +60,7 @@ extern "C" {
 #define EXK_S_DRAIN_TIMEOUT  5  /* in-flight TMA copies did not land within 2 s */
 #define EXK_S_PEER_TIMEOUT   6  /* a peer merge waited > 2 s for another GPU's signal */
 #define EXK_S_PAGE_INDEX     7  /* a block-table entry named a page outside the pool */
-#define EXK_S_POSITION       8  /* a token's position or tail slot, or a length, was out of range */
+#define EXK_S_POSITION       8  /* a token's position or tail slot, a length or a batch's offsets were out of range */
 
 /* One compressed cache (keys or values of one layer): the six buffers of the
  * format above. raw_rows is the number of rows `raw` holds; indices at or
@@ -319,7 +319,8 @@ int exk_attention_bf16_paged(const uint16_t *q, const uint16_t *k, const uint16_
  * fp32 with one rounding to bf16; q_norm and k_norm (bf16 [128], both or
  * neither): each head is first scaled by weight / sqrt(mean square + eps).
  * The rotated queries go to q_out (may be q itself). Rows at and past
- * cu_seqlens[B] are left alone. A token whose position is outside the block
+ * cu_seqlens[B] are left alone, and so are those of a sequence whose offsets
+ * descend or leave [0, N] (not reported). A token whose position is outside the block
  * table or cos_sin is not stored (in a compressed pool none of its sequence's
  * are), its query is written as zeros, and the status word gets
  * EXK_S_POSITION; a block-table entry outside the pool is not written
@@ -382,7 +383,9 @@ int exk_reopen_pages(const int32_t *block_table, int B, int max_pages, int pool_
  * sequence b's at rows [cu_q[b], cu_q[b+1]) (int32, device), its last query at
  * its last key: query i of n sees keys j <= i + L - n of L. A query that sees
  * no key gives zeros; rows at and past cu_q[B] of `out` (strides o_st, o_sh)
- * are left alone. Hq = G * Hkv, G <= 16; at most 65,535 blocks of 2 *
+ * are left alone. Offsets that are no batch's (0 <= cu[0] <= .. <= cu[B] <= rows) are
+ * reported (EXK_S_POSITION): rows of sequences outside [0, N] are not written, of
+ * the others some may not be. Hq = G * Hkv, G <= 16; at most 65,535 blocks of 2 *
  * floor(128 / G) tokens, N / block + B of them (EXK_EARG). ns splits of each row's keys
  * (exk_prefill_splits): with ns > 1 po [N * Hq, ns, 128], pm, pl [N * Hq, ns]
  * fp32 hold their partials. qk_scale: log2(e) / sqrt(128). */

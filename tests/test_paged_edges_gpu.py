@@ -278,3 +278,38 @@ def test_normed_keys_and_queries_one_token_at_a_time():
     some = torch.arange(0, B * n, 97)
     y, tol = rotated(k[some.cuda()], m.cs.cpu()[some % n], w["k_norm"])
     assert ((m.kb[0][at][some.cuda()].double().cpu() - y).abs() <= tol).all()
+
+
+# ----------------------------------------------------------------------------- offsets
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("klen,seqs", [(40, 3), (3000, 3), (3000, 40)])
+def test_offsets_that_are_no_batchs_are_reported_and_leave_rows_alone(klen, seqs):
+    """Rows of a sequence whose offsets leave the batch or descend are not written, with
+    and without splits (where nothing wrote the partials that would be merged), and
+    the call is reported; so are such offsets of the keys."""
+    Hq, Hkv, N = 8, 2, 20
+    lens = [12] + [0] * (seqs - 3) + [4, 4]
+    bad = offsets(lens)
+    bad[-2] = 30                                     # 0, 12, .., 12, 30, 20: past the queries, then descending
+    q, k, v = inputs(N, klen * seqs, Hq, Hkv, seed=42)
+    ck = offsets([klen] * seqs)
+    plan = kernels.lib.exk_prefill_splits(N, seqs, Hq, Hkv, klen, kernels.num_sms())
+    assert (plan > 1) == (klen > 1000)
+    good = offsets(lens)
+    want = ekv.attention_prefill(q, k, v, good, ck)
+    kernels.check_status()
+    junk = torch.full((N * Hq * plan * (D + 2),), float("nan"), device="cuda")
+    del junk                                         # (what the call's workspace may find)
+    hold = torch.full_like(q, 5.0)
+    ekv.attention_prefill(q, k, v, bad, ck, out=hold)
+    assert (hold[12:] == 5).all()
+    assert same_bits(hold[:12], want[:12]) or (hold[:12] == 5).all()
+    with pytest.raises(RuntimeError, match="offsets"):
+        kernels.check_status()
+    for at, x in ((0, -1), (1, 2 * klen + 1), (seqs, klen * seqs + 1)):
+        wrong = ck.clone()
+        wrong[at] = x
+        ekv.attention_prefill(q, k, v, good, wrong)
+        with pytest.raises(RuntimeError, match="offsets"):
+            kernels.check_status()
