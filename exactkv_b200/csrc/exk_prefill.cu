@@ -530,7 +530,9 @@ __device__ __forceinline__ void output_item(const PrefillArgs& a, const Work& w,
     for (int i = 0; i < 32; ++i) f[i] = l == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
     if (bad && valid) {
       // a masked tile held values that are not finite: they were left out of
-      // the product and reach the rows that see them here
+      // the product and reach the rows that see them here, whatever their weight (it is
+      // above 0 in the formula; where it underflows, a product gives NaN instead of
+      // infinity: not finite either way)
 #pragma unroll 1
       for (int t = max(w.low, (w.t1 - w.nt) * kTile); t < min(w.t1 * kTile, lim + 1); ++t) {
         int64_t vrow = static_cast<int64_t>(w.krow) + t;
@@ -938,6 +940,11 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constan
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) den += __shfl_xor_sync(0xFFFFFFFFu, den, d);
+  // Splits that saw a key of the row. (A weight of 0 does not leave one out: its o may be
+  // infinite or NaN, and 0 times that is NaN, as it is without splits.)
+  uint32_t saw[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) saw[i] = __ballot_sync(0xFFFFFFFFu, m[i] != -INFINITY || l[i] != 0.f);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const float4* o = reinterpret_cast<const float4*>(a.po + row * a.ns * kD) + lane;
   for (int s0 = 0; s0 < a.ns; s0 += 8) {
@@ -947,7 +954,7 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constan
     for (int u = 0; u < 8; ++u) {
       g[u] = __shfl_sync(0xFFFFFFFFu, s0 < 32 ? f[0] : f[1], (s0 + u) & 31);
       v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (s0 + u < a.ns && g[u] != 0.f) v[u] = o[(s0 + u) * (kD / 4)];
+      if (((s0 < 32 ? saw[0] : saw[1]) >> ((s0 + u) & 31)) & 1u) v[u] = o[(s0 + u) * (kD / 4)];
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {

@@ -313,3 +313,31 @@ def test_offsets_that_are_no_batchs_are_reported_and_leave_rows_alone(klen, seqs
         ekv.attention_prefill(q, k, v, good, wrong)
         with pytest.raises(RuntimeError, match="offsets"):
             kernels.check_status()
+
+
+# ----------------------------------------------------------------------------- values
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("lens,klens,cold,hot", [
+    ([4], [5000], 10, 4990), ([4], [5000], 4990, 10), ([4], [5000], 2500, 2501), ([300], [300], 10, 200),
+    ([300], [300], 200, 10), ([300], [600], 590, 3)])
+def test_value_that_is_not_finite_under_a_weight_that_vanishes(lens, klens, cold, hot, bad):
+    """Scores 350 apart: the key's weight is exp(-350) in the formula and underflows in 32
+    bits. The rows that see it are not finite in its channel, whatever the tile, the mask
+    and the splits; every other value keeps its bits."""
+    Hq, Hkv, n, L = 8, 2, lens[0], klens[0]
+    q, k, v = inputs(n, L, Hq, Hkv, seed=44)
+    q.zero_(), k.zero_()
+    q[..., 0] = 8
+    k[hot, :, 0] = 500
+    cu, ck = offsets(lens), offsets(klens)
+    clean = ekv.attention_prefill(q, k, v, cu, ck)
+    o, tol = reference(q, k, v, lens, klens)
+    assert ((clean.double().cpu() - o).abs() <= tol).all()
+    v[cold, 1, 77] = bad
+    out = ekv.attention_prefill(q, k, v, cu, ck)
+    hit = torch.zeros(n, Hq, D, dtype=torch.bool, device="cuda")
+    hit[max(0, cold - (L - n)):, 4:, 77] = True
+    assert torch.equal(~torch.isfinite(out.float()), hit)
+    assert same_bits(torch.where(hit, 0, out), torch.where(hit, 0, clean))
