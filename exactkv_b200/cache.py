@@ -290,9 +290,14 @@ class PagedCompressedKV:
         pool moved (a captured graph must be captured again). Raises RuntimeError when
         appends have wanted more raw rows than there were: the pages that had no room
         are lost (readers report them) and their sequences must be appended again."""
-        used = int(self.cnt.item())
-        need = used + (tokens + P * self.pool.nseq) * self.H
-        old = self.pool.cap
+        return self._grow(int(self.cnt.item()), (tokens + P * self.pool.nseq) * self.H)
+
+    def _make_room(self, used, pages):
+        """check_overflow()'s share: room for `pages` worst-case pages of every sequence."""
+        return self._grow(used, pages * P * self.pool.nseq * self.H)
+
+    def _grow(self, used, rows):
+        need, old = used + rows, self.pool.cap
         if used > old:
             raise RuntimeError(f"{used} raw rows appended to a pool of {old}: pages without room were not kept")
         if need <= old:
@@ -328,9 +333,10 @@ class BF16KV:
 def check_overflow(caches):
     """The host check after a page boundary: one sync reads the slot counters of
     all compressed caches (and the kernels' status word, raising on a fault), then
-    every pool with less than one worst-case page free grows. Returns the number
-    of caches that grew."""
-    cs = [c for c in caches if isinstance(c, CompressedKV) and not c._checked]
+    every pool with less than one worst-case page a sequence free grows. Returns the
+    number of caches that grew. A PagedCompressedKV, whose lengths the host does not
+    know, is looked at in every call: one call in 16 steps of a token each is enough."""
+    cs = [c for c in caches if isinstance(c, PagedCompressedKV) or isinstance(c, CompressedKV) and not c._checked]
     if not cs:
         return 0
     status = kernels.status_tensor(cs[0].dev)

@@ -341,3 +341,36 @@ def test_value_that_is_not_finite_under_a_weight_that_vanishes(lens, klens, cold
     hit[max(0, cold - (L - n)):, 4:, 77] = True
     assert torch.equal(~torch.isfinite(out.float()), hit)
     assert same_bits(torch.where(hit, 0, out), torch.where(hit, 0, clean))
+
+
+# ----------------------------------------------------------------------------- growing and cleaning up
+
+@pytest.mark.gpu
+def test_check_overflow_covers_paged_pools():
+    """One call for all layers' pools, contiguous ones among them: those with less than a
+    worst-case page for every sequence grow, and the next 16 steps fit."""
+    Hq, Hkv, B = 4, 2, 3
+    m = Model(B, Hkv, 8, seed=60)
+    for c in (m.kc, m.vc):
+        c.pool = type(c.pool)(B, Hkv, D, 64, c.dev)
+        c._bind()
+    flat = ekv.CompressedKV(B, 64, Hkv, D)
+    new = [5, 14, 16]
+    q, k, v = tokens(sum(new), Hq, Hkv, seed=770)
+    escaping(k, v)
+    grew = ekv.check_overflow([m.kc, flat, m.vc])
+    assert grew == 2 and m.kc.cap >= 16 * B * Hkv and m.kc.pool.moves == 1
+    append_both(m, q, k, v, new, new)
+    lens = new
+    for step in range(40):
+        if step % 16 == 0:
+            ekv.check_overflow([m.kc, m.vc])
+        q, k, v = tokens(B, Hq, Hkv, seed=780 + 3 * step)
+        escaping(k, v, phase=step)
+        lens = [n + 1 for n in lens]
+        append_both(m, q, k, v, lens, [1] * B)
+        assert int(m.vc.cnt.item()) <= m.vc.cap
+    assert int(m.vc.cnt.item()) > 100 and m.vc.pool.moves > 1
+    assert ekv.check_overflow([]) == 0
+    check_same_pools(m, lens)
+    kernels.check_status()
