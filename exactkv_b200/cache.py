@@ -289,8 +289,32 @@ class PagedCompressedKV:
         the rows already in open pages: 16 for each sequence). Returns True when the
         pool moved (a captured graph must be captured again). Raises RuntimeError when
         appends have wanted more raw rows than there were: the pages that had no room
-        are lost (readers report them) and their sequences must be appended again."""
+        are lost (readers report them) and their sequences must be appended again
+        (after compact() without them).
+
+        The reservation is for the worst case, the size of the tokens uncompressed: a long
+        prompt appended in chunks, each after a call of its own, needs less."""
         return self._grow(int(self.cnt.item()), (tokens + P * self.pool.nseq) * self.H)
+
+    def compact(self, block_table):
+        """Gives the raw rows of pages that no sequence uses any more back to the pool:
+        appends only ever take new ones, so a pool whose pages pass from sequence to
+        sequence runs full without it. block_table: int32, any shape, the pages in use
+        (others' contents are lost; entries outside the pool, such as -1, are passed
+        over). Their raw rows move to the front of the pool, whose storage stays where
+        it is: a captured graph stays valid. Syncs. Returns the rows in use."""
+        at = block_table.flatten().long()
+        pages = torch.unique(at[(at >= 0) & (at < self.TS // P)])
+        first = self.rowoff[0, pages].long()                         # [pages in use, H]
+        kept = (first >= 0) & (first < self.pool.cap)                # not open, and not without room
+        rows = (self.rowmask[0, pages, :, None] >> torch.arange(P, device=self.dev) & 1).sum(-1) * kept
+        end = rows.flatten().cumsum(0).view_as(rows)
+        total = int(end[-1, -1]) if len(pages) else 0
+        src = torch.repeat_interleave((first - end + rows).flatten(), rows.flatten(), output_size=total)
+        self.pool.rows[:total] = self.pool.rows[src + torch.arange(total, device=self.dev)]
+        self.rowoff[0, pages] = torch.where(kept, end - rows, first).int()
+        self.cnt.fill_(total)
+        return total
 
     def _make_room(self, used, pages):
         """check_overflow()'s share: room for `pages` worst-case pages of every sequence."""

@@ -374,3 +374,47 @@ def test_check_overflow_covers_paged_pools():
     assert ekv.check_overflow([]) == 0
     check_same_pools(m, lens)
     kernels.check_status()
+
+
+@pytest.mark.gpu
+def test_raw_rows_of_freed_pages_are_given_back():
+    """Sequences come and go on a pool's pages; compact() keeps the raw rows of the pages
+    in use, so the raw pool stays as it is. Open pages and pages shared by two tables
+    are kept, and the storage does not move."""
+    Hq, Hkv = 4, 2
+    m = Model(3, Hkv, 4, seed=64)
+    lens = [0, 0, 0]
+    for c in (m.kc, m.vc):
+        c.ensure_headroom(400)
+    at = [c.pool.rows.data_ptr() for c in (m.kc, m.vc)]
+    for turn in range(12):
+        gone = turn % 3                                  # this sequence ends; its pages and its slot go to another
+        lens[gone] = 0
+        new = [0, 0, 0]
+        new[gone] = 21 + turn
+        new[(gone + 1) % 3] = 1
+        q, k, v = tokens(sum(new), Hq, Hkv, seed=920 + 3 * turn)
+        escaping(k, v, 1 + turn % 2)
+        live = torch.cat([torch.cat([m.table[b, :-(-n // 16)], ints([-1])]) for b, n in enumerate(lens)])
+        live = torch.cat([live, live]).view(2, -1)       # as two tables that share every page
+        for c in (m.kc, m.vc):
+            used = int(c.cnt.item())
+            kept = c.compact(live)
+            assert kept == int(c.cnt.item()) <= used
+        check_same_pools(m, lens)
+        lens = [a + b for a, b in zip(lens, new)]
+        append_both(m, q, k, v, lens, new)
+        check_same_pools(m, lens)
+        assert int(m.vc.cnt.item()) <= 3 * 64 * Hkv
+    assert at == [c.pool.rows.data_ptr() for c in (m.kc, m.vc)]
+    # a pool that ran out goes on without the pages that had no room
+    live = m.table[0, :-(-lens[0] // 16)]
+    m.vc.cnt.fill_(m.vc.cap + 1)
+    with pytest.raises(RuntimeError, match="raw rows"):
+        ekv.check_overflow([m.vc])
+    assert m.vc.compact(live) <= 64 * Hkv and not m.vc.ensure_headroom(64)
+    m.kc.compact(live)
+    check_same_pools(m, lens[:1])
+    for c in (m.kc, m.vc):
+        assert c.compact(m.table[:0]) == 0
+    kernels.check_status()
