@@ -655,6 +655,8 @@ int check_append(const exk_append* t) {
   if (t->N > (1 << 28) || t->B > (1 << 24) || t->Hq > 4096) return EXK_EARG;
   if (!aligned16(t->q) || !aligned16(t->k) || !aligned16(t->v) || !aligned16(t->q_out) || !aligned16(t->cos_sin))
     return EXK_EALIGN;
+  for (const uint16_t* w : {t->q_norm, t->k_norm})  // read 8 bytes at a time
+    if ((reinterpret_cast<uintptr_t>(w) & 7u) != 0) return EXK_EALIGN;
   for (int64_t s : {t->q_st, t->q_sh, t->k_st, t->k_sh, t->v_st, t->v_sh, t->o_st, t->o_sh})
     if (s % 8 != 0) return EXK_EALIGN;
   return 0;

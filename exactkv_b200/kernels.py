@@ -563,8 +563,9 @@ def _append_args(q, k, v, cos_sin, block_table, seq_lens, cu_seqlens, slots, q_n
     wq = wk = 0
     if q_norm is not None:
         for w in (q_norm, k_norm):
-            if w.dtype is not torch.bfloat16 or w.shape != (D,) or w.device != dev or not w.is_contiguous():
-                raise ValueError(f"q_norm and k_norm must be contiguous bf16 tensors [{D}] on {dev}")
+            if w.dtype is not torch.bfloat16 or w.shape != (D,) or w.device != dev or not w.is_contiguous() or \
+                    w.data_ptr() % 8:
+                raise ValueError(f"q_norm and k_norm must be contiguous, 8-byte aligned bf16 tensors [{D}] on {dev}")
         wq, wk = q_norm.data_ptr(), k_norm.data_ptr()
     q_out, (o_at, o_st, o_sh) = _new_rows(q_out, "q_out", q, N, Hq)
     a = APPEND.pack(q_at, k_at, v_at, o_at, q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, cos_sin.data_ptr(), wq, wk,

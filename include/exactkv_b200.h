@@ -316,8 +316,8 @@ int exk_attention_bf16_paged(const uint16_t *q, const uint16_t *k, const uint16_
  * in page block_table[b * max_pages + p / 16] (int32, device). cos_sin: fp32
  * [rope_rows, 128], row p the cosines then the sines of the 64 angles of
  * position p. Queries and keys are rotated (channel j pairs with j + 64) in
- * fp32 with one rounding to bf16; q_norm and k_norm (bf16 [128], both or
- * neither): each head is first scaled by weight / sqrt(mean square + eps).
+ * fp32 with one rounding to bf16; q_norm and k_norm (bf16 [128], 8-byte
+ * aligned, both or neither): each head is first scaled by weight / sqrt(mean square + eps).
  * The rotated queries go to q_out (may be q itself). Rows at and past
  * cu_seqlens[B] are left alone, and so are those of a sequence whose offsets
  * descend or leave [0, N] (not reported). A token whose position is outside the block

@@ -280,6 +280,42 @@ def test_normed_keys_and_queries_one_token_at_a_time():
     assert ((m.kb[0][at][some.cuda()].double().cpu() - y).abs() <= tol).all()
 
 
+def test_norm_weights_off_their_alignment_are_refused():
+    """The kernels read them 8 bytes at a time: a view into a flat buffer of weights may
+    begin anywhere. Refused by the C entries before any launch (addresses never touched)."""
+    import ctypes
+    from exactkv_b200._lib import APPEND, CView, lib
+    at = 1 << 40
+    fits = [at, at, at, at, 1024, 128, 256, 128, 256, 128, 1024, 128, at, at, at, 0, at, at, 0, 4, 4, 8, 2, 64, 4, 16, 1e-6]
+    pools = [ctypes.byref(CView(x, x, x, x, x, x, 1000 + 4 * 32)) for x in (at, 2 * at)]
+    n = lib.exk_rope_append_scratch(4, 4, 2, 0)
+    for which in (13, 14):
+        for off in (2, 4, 6):
+            a = APPEND.pack(*[x + off if i == which else x for i, x in enumerate(fits)])
+            assert lib.exk_rope_append_bf16(a, at, 2 * at, None, 0, None) == -2
+            assert lib.exk_rope_append_compressed(a, pools[0], 1000, at, pools[1], 1000, 2 * at, at, n, None, 0, None) == -2
+
+
+@pytest.mark.gpu
+def test_norm_weights_may_be_aligned_views_and_no_others():
+    Hkv = 2
+    m = Model(1, Hkv, 2, seed=41)
+    q, k, v = tokens(20, 4, Hkv, seed=765)
+    flat = torch.randn(3 * D, device="cuda").to(torch.bfloat16)
+    sl, cu = ints([20]), offsets([20])
+    for off, fits in ((8, True), (4, True), (1, False), (6, False)):
+        w = flat[off:off + D]
+        for call, pools in ((ekv.rope_append_paged, (m.kc, m.vc)), (ekv.rope_append_reference_paged, (m.kb, m.vb))):
+            if not fits:
+                with pytest.raises(ValueError, match="8-byte"):
+                    call(q, k, v, m.cs, *pools, m.table, sl, cu, q_norm=w, k_norm=w)
+                continue
+            got = call(q, k, v, m.cs, *pools, m.table, sl, cu, q_norm=w, k_norm=w)
+            y, tol = rotated(q, m.cs[:20], w)
+            assert ((got.double().cpu() - y).abs() <= tol).all()
+    kernels.check_status()
+
+
 # ----------------------------------------------------------------------------- offsets
 
 @pytest.mark.gpu
