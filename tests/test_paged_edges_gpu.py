@@ -379,6 +379,63 @@ def test_value_that_is_not_finite_under_a_weight_that_vanishes(lens, klens, cold
     assert same_bits(torch.where(hit, 0, out), torch.where(hit, 0, clean))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_channels_beside_a_value_that_is_not_finite_keep_their_bits(bad):
+    Hq, Hkv = 8, 2
+    for lens, klens, at in (([300], [300], 150), ([20, 30], [20, 30], 12), ([4], [5000], 4998), ([4], [5000], 700)):
+        q, k, v = inputs(sum(lens), sum(klens), Hq, Hkv, seed=46)
+        cu, ck = offsets(lens), offsets(klens)
+        clean = ekv.attention_prefill(q, k, v, cu, ck)
+        v[at, 1, 77] = bad
+        out = ekv.attention_prefill(q, k, v, cu, ck)
+        out[:, 4:, 77] = clean[:, 4:, 77]
+        assert same_bits(out, clean)
+
+
+SEEN = [([300], [300]), ([300], [1000]), ([1, 40, 129], [1, 333, 2049]), ([3], [9000]), ([50], [4097]), ([5, 2, 9], [6000, 4095, 1000])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (7, 1), (28, 4)])
+@pytest.mark.parametrize("case", range(len(SEEN)))
+def test_each_row_sees_each_key_once(case, Hq, Hkv):
+    """Scores of zero and values that are 1 in one channel of one key: a row's output is
+    1 / (its keys) in the channels of the keys that it sees, once each, and 0 elsewhere.
+    128 keys at a time: the ends of tiles, pages and splits, the first and the last, and
+    others. With p = 1 and whole sums the only roundings are the quotient's: 2^-8 for
+    bf16, 2^-20 for the 32 bits before it."""
+    lens, klens = SEEN[case]
+    g = torch.Generator().manual_seed(case)
+    N, Nk = sum(lens), sum(klens)
+    m = Model(len(lens), Hkv, -(-max(klens) // 16), seed=50 + case)
+    q = torch.zeros(N, Hq, D, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(Nk, Hkv, D, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    chosen, at = [], 0
+    for n, L in zip(lens, klens):
+        edge = [0, 1, 15, 16, 17, 127, 128, 129, 255, 256, L - 1, L - 2, L - n, L - n - 1, L - n + 1, L - 129, L - 128, L - 17, L - 16]
+        edge += [t * 128 + d for t in range(2, L // 128, max(1, L // 128 // 16)) for d in (-1, 0)]
+        keys = [j for j in dict.fromkeys(edge) if 0 <= j < L][:D]
+        keys += torch.randint(0, L, (D - len(keys),), generator=g).tolist()
+        chosen.append(keys)
+        v[at + torch.tensor(keys), :, torch.arange(D)] = 1
+        at += L
+    want, at = torch.zeros(N, D, dtype=torch.float64), 0
+    for b, (n, L) in enumerate(zip(lens, klens)):
+        last = torch.arange(n) + L - n
+        want[at:at + n] = (torch.tensor(chosen[b])[None] <= last[:, None]).double() / (last + 1)[:, None]
+        at += n
+    cu, ck, sl = offsets(lens), offsets(klens), ints(klens)
+    append_both(m, k, k, v, klens, klens)
+    outs = [ekv.attention_prefill(q, k, v, cu, ck), ekv.attention_prefill_paged(q, m.kc, m.vc, m.table, sl, cu),
+            ekv.attention_prefill_reference_paged(q, m.kb, m.vb, m.table, sl, cu)]
+    for out in outs:
+        err = (out.double().cpu() - want[:, None]).abs()
+        assert (err <= (2.0 ** -8 + 2.0 ** -20) * want[:, None]).all()
+    kernels.check_status()
+
+
 # ----------------------------------------------------------------------------- growing and cleaning up
 
 @pytest.mark.gpu
@@ -409,6 +466,25 @@ def test_check_overflow_covers_paged_pools():
     assert int(m.vc.cnt.item()) > 100 and m.vc.pool.moves > 1
     assert ekv.check_overflow([]) == 0
     check_same_pools(m, lens)
+    kernels.check_status()
+
+
+@pytest.mark.gpu
+def test_growth_moves_open_pages_and_keeps_every_row():
+    Hq, Hkv, lens = 4, 2, [0, 0]
+    m = Model(2, Hkv, 16, seed=62)
+    for c in (m.kc, m.vc):
+        c.pool = type(c.pool)(2, Hkv, D, 64, c.dev)
+        c._bind()
+    for i, new in enumerate(([20, 3], [1, 40], [60, 30])):
+        moved = [c.ensure_headroom(sum(new)) for c in (m.kc, m.vc)]
+        assert moved == [True, True] or i == 1
+        q, k, v = tokens(sum(new), Hq, Hkv, seed=900 + 3 * i)
+        escaping(k, v)
+        lens = [a + b for a, b in zip(lens, new)]
+        append_both(m, q, k, v, lens, new)
+        check_same_pools(m, lens)
+    assert m.kc.pool.moves >= 2
     kernels.check_status()
 
 
