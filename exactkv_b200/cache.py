@@ -303,15 +303,15 @@ class PagedCompressedKV:
         (others' contents are lost; entries outside the pool, such as -1, are passed
         over). Their raw rows move to the front of the pool, whose storage stays where
         it is: a captured graph stays valid. Syncs. Returns the rows in use."""
-        at = block_table.flatten().long()
+        at = block_table.to(self.rowoff.device).flatten().long()
         pages = torch.unique(at[(at >= 0) & (at < self.TS // P)])
         first = self.rowoff[0, pages].long()                         # [pages in use, H]
         kept = (first >= 0) & (first < self.pool.cap)                # not open, and not without room
-        rows = (self.rowmask[0, pages, :, None] >> torch.arange(P, device=self.dev) & 1).sum(-1) * kept
+        rows = (self.rowmask[0, pages, :, None] >> torch.arange(P, device=pages.device) & 1).sum(-1) * kept
         end = rows.flatten().cumsum(0).view_as(rows)
         total = int(end[-1, -1]) if len(pages) else 0
         src = torch.repeat_interleave((first - end + rows).flatten(), rows.flatten(), output_size=total)
-        self.pool.rows[:total] = self.pool.rows[src + torch.arange(total, device=self.dev)]
+        self.pool.rows[:total] = self.pool.rows[src + torch.arange(total, device=pages.device)]
         self.rowoff[0, pages] = torch.where(kept, end - rows, first).int()
         self.cnt.fill_(total)
         return total

@@ -14,7 +14,8 @@
 // Long calls are bound by memory: 11,016 tokens of 32 + 8 + 8 heads into bf16 pages
 // take 44.4 us (276 MB, 6.2 TB/s; with the norm 49 us), 9,529 of 28 + 4 + 4 into
 // coded pages 36 us (14 the encoding, 22 the queries, the raw rows' places beside
-// them); a step of 64 sequences 3 us, of 32 into coded pages 9 us.
+// them; 39 us a call with its launches); a step of 64 sequences 3 us, of 32 into coded
+// pages 9 us.
 #include <algorithm>
 
 #include "exk_device.cuh"

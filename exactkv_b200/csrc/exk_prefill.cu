@@ -20,8 +20,9 @@
 // for its 256 rows; a tile's chain (S out of TMEM 60 cycles, maximum 400,
 // exponentials 1,350, then P V's rest, the next S and the hand-overs 1,150) sets
 // a period of about 3,000, 66 % of the tensor pipe, at the 1.6 GHz that the power
-// limit leaves. One prompt of 16,384 tokens, 32 heads over 8: 1,676 us (1,312
-// TFLOP/s); 4,096: 133 us; 16 prompts of 73 to 1,988 tokens, 28 over 4: 192 us.
+// limit leaves. One prompt of 16,384 tokens, 32 heads over 8: 1,676 us after a pause
+// (1,312 TFLOP/s), 1,952 us in a loop under the power limit; 4,096: 133 and 145 us; 16
+// prompts of 73 to 1,988 tokens, 28 over 4: 192 and 217 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
