@@ -313,6 +313,11 @@ class PagedCompressedKV:
         src = torch.repeat_interleave((first - end + rows).flatten(), rows.flatten(), output_size=total)
         self.pool.rows[:total] = self.pool.rows[src + torch.arange(total, device=pages.device)]
         self.rowoff[0, pages] = torch.where(kept, end - rows, first).int()
+        # (a page that a table names before its sequence comes to it must not claim, at a
+        # later call, the slots that its old rows had)
+        gone = torch.ones(self.TS // P, 1, dtype=torch.bool, device=pages.device)
+        gone[pages] = False
+        self.rowmask[0].masked_fill_(gone, 0)
         self.cnt.fill_(total)
         return total
 

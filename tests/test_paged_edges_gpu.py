@@ -530,3 +530,33 @@ def test_raw_rows_of_freed_pages_are_given_back():
     for c in (m.kc, m.vc):
         assert c.compact(m.table[:0]) == 0
     kernels.check_status()
+
+
+@pytest.mark.gpu
+def test_compact_with_pages_set_aside():
+    """A table may name pages that its sequence has not come to yet. What an earlier sequence
+    left in them is not taken for rows in use once the pool was cleaned up without it: the
+    count never grows, and the open pages behind the capacity are not written over."""
+    Hq, Hkv = 4, 2
+    m = Model(2, Hkv, 4, seed=66)
+    for c in (m.kc, m.vc):
+        c.pool = type(c.pool)(2, Hkv, D, 140, c.dev)
+        c._bind()
+    q, k, v = tokens(64 + 20, Hq, Hkv, seed=960)
+    escaping(k, v)
+    append_both(m, q[:64], k[:64], v[:64], [64, 0], [64, 0])
+    lens = [0, 5]
+    for c in (m.kc, m.vc):
+        assert c.compact(m.table[1]) == 0                # sequence 0 has ended
+    append_both(m, q[64:69], k[64:69], v[64:69], lens, [0, 5])
+    check_same_pools(m, lens)
+    for n in (15, 12, 17):                               # sequence 1 goes on; 0's pages are set aside for another
+        q, k, v = tokens(n, Hq, Hkv, seed=970 + n)
+        escaping(k, v)
+        lens = [0, lens[1] + n]
+        append_both(m, q, k, v, lens, [0, n])
+        for c in (m.kc, m.vc):
+            used = int(c.cnt.item())
+            assert c.compact(m.table) <= used
+        check_same_pools(m, lens)
+    kernels.check_status()
